@@ -26,8 +26,8 @@
 
 using namespace gl3;
 
-static std::string g_create_err;
-void gl3_set_create_error(const char* msg) { g_create_err = msg ? msg : ""; }
+static thread_local std::string g_create_err;          // of the calling thread: operators are called from several at once
+void gl3_set_create_error(const char* msg) { try { g_create_err = msg ? msg : ""; } catch (...) { g_create_err.clear(); } }
 
 static double now_ms() {
     return std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now().time_since_epoch()).count();

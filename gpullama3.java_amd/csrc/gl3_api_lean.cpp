@@ -5,8 +5,8 @@
 
 #include "gl3_hy_dispatch.h"
 
-static std::string g_create_err;
-void gl3_set_create_error(const char* msg) { g_create_err = msg ? msg : ""; }
+static thread_local std::string g_create_err;          // of the calling thread: operators are called from several at once
+void gl3_set_create_error(const char* msg) { try { g_create_err = msg ? msg : ""; } catch (...) { g_create_err.clear(); } }
 int32_t gl3_tp_check(gl3_ctx*) { return GL3_OK; }          // no tensor-parallel transport in this build
 
 #define LEAN_CTX(c) do { if (!(c)) return GL3_E_ARG; if (!(c)->hy) return GL3_E_UNSUPPORTED; } while (0)

@@ -1,0 +1,193 @@
+// gl3_ops.hip — operators on the caller's device memory: int8 rows, their products, log probabilities of tokens.  Argument checks, launches.
+#include "gl3_ops.h"
+
+#include <algorithm>
+#include <climits>
+
+#include "gl3_ops_int8.h"
+#include "gl3_ops_logprobs.h"
+
+void gl3_set_create_error(const char* msg);
+
+static inline int64_t op_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+template <typename F> static void op_with_type(int32_t type, F&& f) {
+    if (type == GL3_TYPE_F32) f(float{}); else if (type == GL3_TYPE_F16) f(__half{}); else f(op_bf16{});
+}
+
+// ---- launches -------------------------------------------------------------------------------------------------------------------------
+void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale) {
+    op_with_type(type, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((op_quantize_kernel<T>), dim3((unsigned)rows), dim3(256), 0, s, (const T*)x, cols, ldx, codes, ldq, scale);
+    });
+}
+
+uint64_t op_product_workspace(int64_t, int64_t, int32_t) { return 0; }
+void op_product(hipStream_t s, const OpProduct& p, void*) {
+    op_with_type(p.y_type, [&](auto t) {
+        typedef decltype(t) TY;
+        constexpr int64_t GY = 65535;          // grids of more row tiles go in pieces
+        for (int64_t m0 = 0; m0 < p.m; m0 += GY * 16) {
+            const int64_t m = std::min(p.m - m0, GY * 16);
+            hipLaunchKernelGGL((op_product_kernel<TY>), dim3((unsigned)op_cdiv(p.n, 16), (unsigned)op_cdiv(m, 16)), dim3(64), 0, s, p.a + m0 * p.lda, p.lda, p.a_scale + m0, p.w, p.ldw,
+                               p.w_scale, p.bias, m, p.n, p.k, (TY*)p.y + m0 * p.ldy, p.ldy);
+        }
+    });
+}
+
+// workspace of a linear: codes of the rows, their scales, then what the product needs
+static uint64_t op_linear_codes(int64_t m, int32_t k) { return (uint64_t)m * op_code_ld(k); }
+static uint64_t op_linear_rows(int64_t m, int32_t k) { return op_linear_codes(m, k) + (uint64_t)op_cdiv(m, 4) * 16; }
+uint64_t op_linear_workspace(int64_t m, int64_t n, int32_t k) { return op_linear_rows(m, k) + op_product_workspace(m, n, k); }
+void op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const OpProduct& p, void* workspace) {
+    OpProduct q = p;
+    int8_t* codes = (int8_t*)workspace;
+    float* scale = (float*)(codes + op_linear_codes(p.m, p.k));
+    q.a = codes; q.lda = op_code_ld(p.k); q.a_scale = scale;
+    op_quantize(s, x, x_type, p.m, p.k, ldx, codes, q.lda, scale);
+    op_product(s, q, (uint8_t*)workspace + op_linear_rows(p.m, p.k));
+}
+
+uint64_t op_logprobs_workspace(int64_t, int32_t, int32_t) { return 0; }
+void op_logprobs(hipStream_t s, const OpLogprobs& p, void*) {
+    op_with_type(p.type, [&](auto t) {
+        typedef decltype(t) T;
+        hipLaunchKernelGGL((op_logprobs_kernel<T>), dim3((unsigned)p.rows), dim3(256), 0, s, (const T*)p.logits, p.vocab, p.ld, p.targets, p.top, p.logprob, p.rank, p.entropy, p.top_ids,
+                           p.top_logprobs);
+    });
+}
+
+// ---- entry points ---------------------------------------------------------------------------------------------------------------------
+namespace {
+int32_t refuse(int32_t code, const char* msg) { gl3_set_create_error(msg); return code; }
+#define OP_ARG(cond, msg) do { if (!(cond)) return refuse(GL3_E_ARG, msg); } while (0)
+
+bool float_type(int32_t t) { return t == GL3_TYPE_F32 || t == GL3_TYPE_F16 || t == GL3_TYPE_BF16; }
+int type_size(int32_t t) { return t == GL3_TYPE_F32 ? 4 : 2; }
+bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
+// rows of `cols` elements, `ld` apart (one row: any ld): whether their bytes fit an address
+bool rows_ok(int64_t rows, int64_t cols, int64_t ld) { return rows <= 1 || (ld >= cols && ld <= (INT64_MAX >> 4) / rows); }
+
+// the caller's device for the length of a call
+struct OnDevice {
+    int before = -1;
+    bool changed = false;
+    const char* enter(int32_t device, hipStream_t s) {
+        if (device < 0 || hipGetDevice(&before) != hipSuccess) { (void)hipGetLastError(); return "no such device"; }
+        if (before != device) {
+            if (hipSetDevice(device) != hipSuccess) { (void)hipGetLastError(); return "no such device"; }
+            changed = true;
+        }
+        int on = device;
+        if (s && hipStreamGetDevice(s, &on) != hipSuccess) { (void)hipGetLastError(); return "the stream is not valid"; }
+        return on == device ? nullptr : "the stream belongs to another device";
+    }
+    ~OnDevice() { if (changed) (void)hipSetDevice(before); }
+};
+int32_t launched() {
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess ? GL3_OK : refuse(e == hipErrorOutOfMemory ? GL3_E_OOM : GL3_E_HIP, hipGetErrorString(e));
+}
+int32_t check_product(const OpProduct& p) {
+    OP_ARG(p.k >= 1 && p.k <= GL3_INT8_MAX_K, "k out of range (1 .. GL3_INT8_MAX_K)");
+    OP_ARG(p.m >= 0 && p.n >= 0 && p.m <= INT32_MAX && p.n <= INT32_MAX, "m or n out of range");
+    OP_ARG(float_type(p.y_type), "results are GL3_TYPE_F32, F16 or BF16");
+    if (p.m == 0 || p.n == 0) return GL3_OK;
+    OP_ARG(p.w && p.w_scale && p.y, "null pointer");
+    OP_ARG(aligned(p.w, 16) && p.ldw % 16 == 0, "codes start on 16 bytes, and so does every row of them");
+    OP_ARG(rows_ok(p.n, op_code_ld(p.k), p.ldw), "ldw: a row of codes is k columns and zeros up to a multiple of GL3_CODE_BLOCK");
+    OP_ARG(aligned(p.w_scale, 4) && aligned(p.bias, 4) && aligned(p.y, type_size(p.y_type)), "misaligned pointer");
+    OP_ARG(rows_ok(p.m, p.n, p.ldy), "ldy is less than n");
+    return GL3_OK;
+}
+int32_t check_workspace(const void* workspace, uint64_t have, uint64_t need) {
+    OP_ARG(have >= need && (workspace || need == 0), "workspace too small");
+    OP_ARG(need == 0 || aligned(workspace, 16), "the workspace starts on 16 bytes");
+    return GL3_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int32_t gl3_quantize_rows(int32_t device, void* stream, const void* x, int32_t x_type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale) {
+    OP_ARG(float_type(x_type), "rows are GL3_TYPE_F32, F16 or BF16");
+    OP_ARG(rows >= 0 && rows <= INT32_MAX, "rows out of range");
+    OP_ARG(cols >= 1 && cols <= GL3_INT8_MAX_K, "cols out of range (1 .. GL3_INT8_MAX_K)");
+    if (rows == 0) return GL3_OK;
+    OP_ARG(x && codes && scale, "null pointer");
+    OP_ARG(aligned(x, type_size(x_type)) && aligned(scale, 4), "misaligned pointer");
+    OP_ARG(rows_ok(rows, cols, ldx), "ldx is less than cols");
+    OP_ARG(aligned(codes, 16) && ldq % 16 == 0, "codes start on 16 bytes, and so does every row of them");
+    OP_ARG(rows_ok(rows, op_code_ld(cols), ldq), "ldq: a row of codes is cols columns and zeros up to a multiple of GL3_CODE_BLOCK");
+    OnDevice on;
+    if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
+    op_quantize((hipStream_t)stream, x, x_type, rows, cols, ldx, codes, ldq, scale);
+    return launched();
+}
+
+int32_t gl3_int8_workspace(int64_t m, int64_t n, int32_t k, uint64_t* matmul_bytes, uint64_t* linear_bytes) {
+    OP_ARG(k >= 1 && k <= GL3_INT8_MAX_K && m >= 0 && n >= 0 && m <= INT32_MAX && n <= INT32_MAX, "sizes out of range");
+    const bool none = m == 0 || n == 0;
+    if (matmul_bytes) *matmul_bytes = none ? 0 : op_product_workspace(m, n, k);
+    if (linear_bytes) *linear_bytes = none ? 0 : op_linear_workspace(m, n, k);
+    return GL3_OK;
+}
+
+int32_t gl3_int8_matmul(int32_t device, void* stream, const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias, int64_t m,
+                        int64_t n, int32_t k, void* y, int32_t y_type, int64_t ldy, void* workspace, uint64_t workspace_bytes) {
+    const OpProduct p{a, lda, a_scale, w, ldw, w_scale, bias, m, n, k, y, y_type, ldy};
+    int32_t r = check_product(p);
+    if (r != GL3_OK || m == 0 || n == 0) return r;
+    OP_ARG(a && a_scale, "null pointer");
+    OP_ARG(aligned(a, 16) && lda % 16 == 0, "codes start on 16 bytes, and so does every row of them");
+    OP_ARG(rows_ok(m, op_code_ld(k), lda) && aligned(a_scale, 4), "lda: a row of codes is k columns and zeros up to a multiple of GL3_CODE_BLOCK");
+    if ((r = check_workspace(workspace, workspace_bytes, op_product_workspace(m, n, k))) != GL3_OK) return r;
+    OnDevice on;
+    if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
+    op_product((hipStream_t)stream, p, workspace);
+    return launched();
+}
+
+int32_t gl3_int8_linear(int32_t device, void* stream, const void* x, int32_t x_type, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias, int64_t m, int64_t n,
+                        int32_t k, void* y, int32_t y_type, int64_t ldy, void* workspace, uint64_t workspace_bytes) {
+    const OpProduct p{nullptr, 0, nullptr, w, ldw, w_scale, bias, m, n, k, y, y_type, ldy};
+    OP_ARG(float_type(x_type), "rows are GL3_TYPE_F32, F16 or BF16");
+    int32_t r = check_product(p);
+    if (r != GL3_OK || m == 0 || n == 0) return r;
+    OP_ARG(x && aligned(x, type_size(x_type)), "x is null or misaligned");
+    OP_ARG(rows_ok(m, k, ldx), "ldx is less than k");
+    if ((r = check_workspace(workspace, workspace_bytes, op_linear_workspace(m, n, k))) != GL3_OK) return r;
+    OnDevice on;
+    if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
+    op_linear((hipStream_t)stream, x, x_type, ldx, p, workspace);
+    return launched();
+}
+
+int32_t gl3_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top, uint64_t* bytes) {
+    OP_ARG(bytes, "null pointer");
+    OP_ARG(rows >= 0 && rows <= INT32_MAX && vocab >= 1 && top >= 0 && top <= GL3_LOGPROBS_MAX_TOP, "sizes out of range");
+    *bytes = rows == 0 ? 0 : op_logprobs_workspace(rows, vocab, top);
+    return GL3_OK;
+}
+
+int32_t gl3_token_logprobs(int32_t device, void* stream, const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t ld, const int32_t* targets, int32_t top, float* logprob,
+                           int32_t* rank, float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace, uint64_t workspace_bytes) {
+    OP_ARG(float_type(type), "logits are GL3_TYPE_F32, F16 or BF16");
+    OP_ARG(rows >= 0 && rows <= INT32_MAX && vocab >= 1, "rows or vocab out of range");
+    OP_ARG(top >= 0 && top <= GL3_LOGPROBS_MAX_TOP, "top out of range (0 .. GL3_LOGPROBS_MAX_TOP)");
+    OP_ARG((targets != nullptr) == (logprob != nullptr) && (targets != nullptr) == (rank != nullptr), "targets, logprob and rank: all or none");
+    if (rows == 0) return GL3_OK;
+    OP_ARG(logits && aligned(logits, type_size(type)), "logits are null or misaligned");
+    OP_ARG(rows_ok(rows, vocab, ld), "ld is less than vocab");
+    OP_ARG(top == 0 || (top_ids && top_logprobs), "top > 0 needs top_ids and top_logprobs");
+    OP_ARG(aligned(targets, 4) && aligned(logprob, 4) && aligned(rank, 4) && aligned(entropy, 4) && aligned(top_ids, 4) && aligned(top_logprobs, 4), "misaligned pointer");
+    int32_t r = check_workspace(workspace, workspace_bytes, op_logprobs_workspace(rows, vocab, top));
+    if (r != GL3_OK) return r;
+    if (!targets && !entropy && top == 0) return GL3_OK;
+    OnDevice on;
+    if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
+    op_logprobs((hipStream_t)stream, OpLogprobs{logits, type, rows, vocab, ld, targets, top, logprob, rank, entropy, top_ids, top_logprobs}, workspace);
+    return launched();
+}
+
+}  // extern "C"

@@ -153,6 +153,15 @@ _SIGS = {  # symbol -> (restype, argtypes): exactly the declarations of include/
     "gl3_load_model_dir": (C.c_int32, [C.c_char_p, C.POINTER(ModelDesc), C.POINTER(C.c_void_p)]),
     "gl3_is_model_dir": (C.c_int32, [C.c_char_p]),
     "gl3_get_model_desc": (C.c_int32, [C.c_void_p, C.POINTER(ModelDesc)]),
+    "gl3_quantize_rows": (C.c_int32, [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p]),
+    "gl3_int8_matmul": (C.c_int32, [C.c_int32, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                    C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_uint64]),
+    "gl3_int8_linear": (C.c_int32, [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_int64, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64,
+                                    C.c_int32, C.c_void_p, C.c_int32, C.c_int64, C.c_void_p, C.c_uint64]),
+    "gl3_int8_workspace": (C.c_int32, [C.c_int64, C.c_int64, C.c_int32, C.POINTER(C.c_uint64), C.POINTER(C.c_uint64)]),
+    "gl3_token_logprobs": (C.c_int32, [C.c_int32, C.c_void_p, C.c_void_p, C.c_int32, C.c_int64, C.c_int32, C.c_int64, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p,
+                                       C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_uint64]),
+    "gl3_logprobs_workspace": (C.c_int32, [C.c_int64, C.c_int32, C.c_int32, C.POINTER(C.c_uint64)]),
     "gl3_profile_hybrid_gemm": (C.c_int32, [C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.c_int32, C.POINTER(C.c_double)]),
 }
 

@@ -609,6 +609,51 @@ GL3_API int32_t gl3_get_model_desc(gl3_ctx* ctx, gl3_model_desc* desc);
  * Several copies of the matrix are used in rotation so that no launch finds its weights in a cache.  out_us: mean per launch. */
 GL3_API int32_t gl3_profile_hybrid_gemm(int32_t device, int32_t f32, int32_t rows, int32_t k, int32_t m, int32_t glu, int32_t iters, double* out_us);
 
+/* ---- operators on the caller's device memory (csrc/gl3_ops.hip): rows in 8-bit integers, their products, log probabilities of tokens.
+ * They need no plan.  `device` is the HIP ordinal the pointers belong to, `stream` a hipStream_t of that device (NULL: its default stream);
+ * the calling thread's current device is left as it was.  A call returns when its kernels are enqueued, allocates nothing and may be captured
+ * into a graph; results and `workspace` (scratch the caller owns, as many bytes as the *_workspace function of the same sizes says, 16-byte
+ * aligned, NULL where that is 0) belong to the call until the stream has passed it, so calls that may run at the same time need workspaces of
+ * their own, and so do two graphs that may be replayed at the same time.  Outputs must not overlap inputs or each other.  Row strides (ld*) count
+ * elements.  0 rows: nothing to do.  Errors: gl3_last_error(NULL), of the calling thread; nothing has been enqueued when arguments are refused. */
+
+/* rows x cols values of GL3_TYPE_F32 / GL3_TYPE_F16 / GL3_TYPE_BF16 -> int8 codes and one float32 scale per row: x = code * scale within half a
+ * step.  With a = max |x| of the row: scale = a / 127, code = rint(x * (127 / a)), every operation rounded to float32 (a code is the same bits
+ * wherever it is computed so).  a < 2^-100: scale 0, codes 0.  A row that holds a NaN or an infinity: scale NaN, codes 0 (its products are NaN).
+ * A row of codes ends on a multiple of GL3_CODE_BLOCK, zeros behind the last column: ldq >= that and a multiple of 16, codes 16-byte aligned.
+ * Tokens and channels are quantised alike: a weight matrix [out][in] gives its codes and its scale per channel.  1 <= cols <= GL3_INT8_MAX_K. */
+#define GL3_CODE_BLOCK 128
+#define GL3_INT8_MAX_K 131071
+GL3_API int32_t gl3_quantize_rows(int32_t device, void* stream, const void* x, int32_t x_type, int64_t rows, int32_t cols, int64_t ldx,
+                                  int8_t* codes, int64_t ldq, float* scale);
+/* y[i][j] = (float(sum_k a[i][k] w[j][k]) * a_scale[i]) * w_scale[j] (+ bias[j]): m rows of codes against n channels of codes, both as
+ * gl3_quantize_rows lays them out (16-byte aligned, strides multiples of 16, zeros from column k to the next multiple of GL3_CODE_BLOCK); the sum
+ * is exact in int32, whatever the codes (k <= GL3_INT8_MAX_K).  bias: float32 or NULL.  y: GL3_TYPE_F32 / F16 / BF16, one rounding.  m, n < 2^31. */
+GL3_API int32_t gl3_int8_matmul(int32_t device, void* stream, const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw,
+                                const float* w_scale, const float* bias, int64_t m, int64_t n, int32_t k, void* y, int32_t y_type, int64_t ldy,
+                                void* workspace, uint64_t workspace_bytes);
+/* The same for float rows, quantised inside the call: gl3_quantize_rows(x), then gl3_int8_matmul, bit for bit. */
+GL3_API int32_t gl3_int8_linear(int32_t device, void* stream, const void* x, int32_t x_type, int64_t ldx, const int8_t* w, int64_t ldw,
+                                const float* w_scale, const float* bias, int64_t m, int64_t n, int32_t k, void* y, int32_t y_type, int64_t ldy,
+                                void* workspace, uint64_t workspace_bytes);
+/* Bytes of workspace of the two (either pointer may be NULL). */
+GL3_API int32_t gl3_int8_workspace(int64_t m, int64_t n, int32_t k, uint64_t* matmul_bytes, uint64_t* linear_bytes);
+
+/* rows of logits [rows][ld >= vocab] (GL3_TYPE_F32 / F16 / BF16).  With lse = ln sum_v e^x_v of the row, and tokens ordered by falling logit, lower
+ * id first among equals:
+ *   logprob[r]      x_t - lse of the given token t = targets[r], rank[r] its place in that order (1 = most probable); a negative target: none is
+ *                   given, 0 and rank 0; a target >= vocab: NaN and rank 0.  targets, logprob and rank: all or none (NULL).
+ *   entropy[r]      -sum_v p_v ln p_v (NULL: not wanted)
+ *   top_ids[r][top], top_logprobs[r][top]   the first `top` tokens of the order (0 <= top <= GL3_LOGPROBS_MAX_TOP); behind the last token of
+ *                   non-zero probability (logit above -inf): id -1, -inf.
+ * A logit of -inf has probability 0 and adds nothing.  A row of nothing but -inf: log probabilities -inf, entropy 0, no alternatives.  A row that
+ * holds a NaN or +inf has NaN log probabilities and entropy; a NaN is never an alternative and no NaN target has a rank (0).  Sums are float32. */
+#define GL3_LOGPROBS_MAX_TOP 64
+GL3_API int32_t gl3_token_logprobs(int32_t device, void* stream, const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t ld,
+                                   const int32_t* targets, int32_t top, float* logprob, int32_t* rank, float* entropy, int32_t* top_ids,
+                                   float* top_logprobs, void* workspace, uint64_t workspace_bytes);
+GL3_API int32_t gl3_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top, uint64_t* bytes);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,130 @@
+"""Operators on device memory: every refusal of the C entry points, before anything touches a GPU; workspace sizes; the Python twin's own checks."""
+import ctypes as C
+from importlib import import_module
+
+import pytest
+import torch
+
+import __graft_entry__ as ge
+
+
+@pytest.fixture(scope="module")
+def hip(pkg):
+    return import_module(ge.PKG_NAME + ".hip")
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    return import_module(ge.PKG_NAME + ".ops")
+
+
+A = 1 << 20            # an address that is 16-byte aligned and never followed
+B = A + 1
+
+
+def quantize(**kw):
+    a = dict(device=0, stream=None, x=A, type=0, rows=2, cols=5, ldx=5, codes=A, ldq=128, scale=A)
+    a.update(kw)
+    return list(a.values())
+
+
+def matmul(**kw):
+    a = dict(device=0, stream=None, a=A, lda=128, a_scale=A, w=A, ldw=128, w_scale=A, bias=None, m=2, n=3, k=5, y=A, y_type=0, ldy=3, workspace=A, bytes=1 << 30)
+    a.update(kw)
+    return list(a.values())
+
+
+def linear(**kw):
+    a = dict(device=0, stream=None, x=A, x_type=0, ldx=5, w=A, ldw=128, w_scale=A, bias=None, m=2, n=3, k=5, y=A, y_type=0, ldy=3, workspace=A, bytes=1 << 30)
+    a.update(kw)
+    return list(a.values())
+
+
+def logprobs(**kw):
+    a = dict(device=0, stream=None, logits=A, type=0, rows=2, vocab=9, ld=9, targets=A, top=3, logprob=A, rank=A, entropy=A, top_ids=A, top_logprobs=A, workspace=A, bytes=1 << 30)
+    a.update(kw)
+    return list(a.values())
+
+
+BAD = [("gl3_quantize_rows", quantize, kw) for kw in (
+    dict(type=2), dict(type=8), dict(rows=-1), dict(rows=1 << 31), dict(cols=0), dict(cols=-3), dict(cols=131072, ldx=131072, ldq=131072), dict(x=None), dict(codes=None), dict(scale=None),
+    dict(x=B), dict(type=1, x=B), dict(scale=A + 2), dict(ldx=4), dict(ldx=-5), dict(ldx=1 << 62), dict(codes=A + 8), dict(ldq=120), dict(ldq=136), dict(ldq=0), dict(device=-1))]
+BAD += [(name, make, kw) for name, make in (("gl3_int8_matmul", matmul), ("gl3_int8_linear", linear)) for kw in (
+    dict(k=0), dict(k=131072), dict(m=-1), dict(n=-1), dict(m=1 << 31), dict(n=1 << 31), dict(y_type=8), dict(y_type=-1), dict(w=None), dict(w_scale=None), dict(y=None), dict(w=A + 4),
+    dict(ldw=120), dict(ldw=0), dict(ldw=136), dict(w_scale=B), dict(bias=A + 2), dict(y=A + 2), dict(y_type=1, y=B), dict(ldy=2), dict(ldy=1 << 62), dict(device=-1))]
+BAD += [("gl3_int8_matmul", matmul, kw) for kw in (dict(a=None), dict(a_scale=None), dict(a=A + 8), dict(lda=5), dict(lda=0), dict(a_scale=B),
+                                                   dict(k=129, lda=256), dict(k=129, ldw=256))]
+BAD += [("gl3_int8_linear", linear, kw) for kw in (dict(x=None), dict(x=B), dict(x_type=1, x=B), dict(x_type=8), dict(ldx=4), dict(ldx=0), dict(k=129, ldx=129), dict(m=200, workspace=None),
+                                                   dict(m=200, workspace=A + 8), dict(m=200, bytes=0), dict(m=200, bytes=100))]
+BAD += [("gl3_token_logprobs", logprobs, kw) for kw in (
+    dict(type=8), dict(rows=-1), dict(rows=1 << 31), dict(vocab=0), dict(vocab=-1), dict(top=-1), dict(top=65), dict(targets=None), dict(logprob=None), dict(rank=None),
+    dict(targets=None, rank=None), dict(logits=None), dict(logits=B), dict(type=1, logits=B), dict(ld=8), dict(ld=-9), dict(top_ids=None), dict(top_logprobs=None), dict(targets=B),
+    dict(logprob=B), dict(rank=B), dict(entropy=B), dict(top_ids=B), dict(top_logprobs=B), dict(device=-1))]
+
+
+@pytest.mark.parametrize("i", range(len(BAD)))
+def test_refused(hip, i):
+    name, make, kw = BAD[i]
+    assert getattr(hip.lib(), name)(*make(**kw)) == hip.E_ARG, (name, kw)
+    assert hip.lib().gl3_last_error(None), (name, kw)
+
+
+def test_nothing_to_do(hip):
+    L = hip.lib()
+    none = dict(x=None, codes=None, scale=None)
+    assert L.gl3_quantize_rows(*quantize(rows=0, **none)) == 0
+    for m, n in ((0, 3), (2, 0), (0, 0)):
+        assert L.gl3_int8_matmul(*matmul(m=m, n=n, a=None, a_scale=None, w=None, w_scale=None, y=None, workspace=None, bytes=0)) == 0
+        assert L.gl3_int8_linear(*linear(m=m, n=n, x=None, w=None, w_scale=None, y=None, workspace=None, bytes=0)) == 0
+    assert L.gl3_token_logprobs(*logprobs(rows=0, logits=None, workspace=None, bytes=0)) == 0
+
+
+def test_workspace_sizes(hip):
+    L = hip.lib()
+    a, b, c = C.c_uint64(7), C.c_uint64(7), C.c_uint64(7)
+    assert L.gl3_int8_workspace(0, 5, 9, C.byref(a), C.byref(b)) == 0 and (a.value, b.value) == (0, 0)
+    for m, n, k in ((1, 1, 1), (5, 300, 1000), (512, 128256, 4096), (2 ** 31 - 1, 2 ** 31 - 1, 131071)):
+        assert L.gl3_int8_workspace(m, n, k, C.byref(a), C.byref(b)) == 0
+        assert L.gl3_int8_workspace(m, n, k, None, None) == 0
+        assert a.value <= b.value < 2 ** 63
+    for bad in ((-1, 1, 1), (1, -1, 1), (1, 1, 0), (1, 1, 131072), (2 ** 31, 1, 1)):
+        assert L.gl3_int8_workspace(*bad, C.byref(a), C.byref(b)) == hip.E_ARG
+    assert L.gl3_logprobs_workspace(0, 9, 3, C.byref(c)) == 0 and c.value == 0
+    for bad in ((-1, 9, 3), (1, 0, 3), (1, 9, -1), (1, 9, 65)):
+        assert L.gl3_logprobs_workspace(*bad, C.byref(c)) == hip.E_ARG
+    assert L.gl3_logprobs_workspace(1, 9, 3, None) == hip.E_ARG
+
+
+def test_python_checks(hip, ops):
+    x = torch.zeros(2, 5)
+    with pytest.raises(hip.Gl3Error):
+        ops.quantize_rows(x)
+    with pytest.raises(hip.Gl3Error):
+        ops.token_logprobs(x)
+    w = ops.Int8Rows(torch.zeros(3, 128, dtype=torch.int8), torch.ones(3), 5)
+    with pytest.raises(hip.Gl3Error):
+        ops.int8_linear(x, w)
+    with pytest.raises(hip.Gl3Error):
+        ops.int8_matmul(w, w)
+    assert torch.equal(w.dequantize(), torch.zeros(3, 5))
+    assert (ops.CODE_BLOCK, ops.MAX_K, ops.MAX_TOP) == (128, 131071, 64)
+
+
+def test_errors_belong_to_the_thread(hip):
+    """Two threads' refused calls do not touch each other's message."""
+    import threading
+    L = hip.lib()
+    seen = {}
+
+    def work(i):
+        for _ in range(300):
+            bad = logprobs(top=65) if i % 2 else quantize(cols=0)
+            assert (L.gl3_token_logprobs if i % 2 else L.gl3_quantize_rows)(*bad) == hip.E_ARG
+            seen.setdefault(i, set()).add(L.gl3_last_error(None))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert all(len(v) == 1 for v in seen.values()) and len(seen) == 4
+    assert all((b"top" in next(iter(v))) == bool(i % 2) for i, v in seen.items())
