@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "gl3_ops_int8.h"
 #include "gl3_ops_logprobs.h"
@@ -10,6 +11,7 @@
 void gl3_set_create_error(const char* msg);
 
 static inline int64_t op_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+constexpr int64_t OP_GRID = 1 << 22;          // workgroups of one launch, at most (a launch has fewer than 2^32 threads)
 template <typename F> static void op_with_type(int32_t type, F&& f) {
     if (type == GL3_TYPE_F32) f(float{}); else if (type == GL3_TYPE_F16) f(__half{}); else f(op_bf16{});
 }
@@ -18,7 +20,8 @@ template <typename F> static void op_with_type(int32_t type, F&& f) {
 void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale) {
     op_with_type(type, [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((op_quantize_kernel<T>), dim3((unsigned)rows), dim3(256), 0, s, (const T*)x, cols, ldx, codes, ldq, scale);
+        for (int64_t r = 0; r < rows; r += OP_GRID)
+            hipLaunchKernelGGL((op_quantize_kernel<T>), dim3((unsigned)std::min<int64_t>(OP_GRID, rows - r)), dim3(256), 0, s, (const T*)x + r * ldx, cols, ldx, codes + r * ldq, ldq, scale + r);
     });
 }
 
@@ -48,12 +51,34 @@ void op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const 
     op_product(s, q, (uint8_t*)workspace + op_linear_rows(p.m, p.k));
 }
 
-uint64_t op_logprobs_workspace(int64_t, int32_t, int32_t) { return 0; }
-void op_logprobs(hipStream_t s, const OpLogprobs& p, void*) {
+// Parts of a row: as many as give the launch OP_LP_WGS workgroups, none shorter than a small batch, at most 64 (one lane each joins them).
+constexpr int OP_LP_WGS = 1024, OP_LP_SMALL = 2048, OP_LP_BIG = 8192;          // logits of a workgroup's batch
+struct OpLpPlan { int parts, per; bool big; };          // per: logits of a part
+static OpLpPlan op_lp_plan(int64_t rows, int32_t vocab) {
+    const int64_t want = std::min<int64_t>(64, std::max<int64_t>(1, OP_LP_WGS / rows));
+    int64_t per = op_cdiv(op_cdiv(vocab, want), OP_LP_SMALL) * OP_LP_SMALL;
+    const bool big = per >= OP_LP_BIG;
+    if (big) per = op_cdiv(per, OP_LP_BIG) * OP_LP_BIG;
+    return OpLpPlan{(int)op_cdiv(vocab, per), (int)std::min<int64_t>(per, INT32_MAX - OP_LP_BIG + 1), big};
+}
+uint64_t op_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top) {
+    const OpLpPlan pl = op_lp_plan(rows, vocab);
+    return pl.parts == 1 ? 0 : (uint64_t)rows * pl.parts * op_part_bytes(top);
+}
+void op_logprobs(hipStream_t s, const OpLogprobs& p, void* workspace) {
+    const OpRowOut o{p.targets, p.top, p.logprob, p.rank, p.entropy, p.top_ids, p.top_logprobs};
+    const OpLpPlan pl = op_lp_plan(p.rows, p.vocab);
     op_with_type(p.type, [&](auto t) {
         typedef decltype(t) T;
-        hipLaunchKernelGGL((op_logprobs_kernel<T>), dim3((unsigned)p.rows), dim3(256), 0, s, (const T*)p.logits, p.vocab, p.ld, p.targets, p.top, p.logprob, p.rank, p.entropy, p.top_ids,
-                           p.top_logprobs);
+        constexpr int V = 16 / (int)sizeof(T), NT = OP_LP_THREADS;
+        for (int64_t r = 0; r < p.rows; r += 65535) {          // (a grid's y)
+            const dim3 grid((unsigned)pl.parts, (unsigned)std::min<int64_t>(65535, p.rows - r));
+#define OP_LP(U, TOP) hipLaunchKernelGGL((op_logprobs_kernel<T, U, TOP>), grid, dim3(NT), 0, s, (const T*)p.logits, p.vocab, p.ld, r, pl.per / V, o, (uint8_t*)workspace)
+            if (pl.big) { if (p.top) OP_LP(OP_LP_BIG / NT / V, true); else OP_LP(OP_LP_BIG / NT / V, false); }
+            else { if (p.top) OP_LP(OP_LP_SMALL / NT / V, true); else OP_LP(OP_LP_SMALL / NT / V, false); }
+#undef OP_LP
+        }
+        if (pl.parts > 1) hipLaunchKernelGGL((op_logprobs_join_kernel<T>), dim3((unsigned)p.rows), dim3(64), 0, s, (const T*)p.logits, p.vocab, p.ld, pl.parts, o, (const uint8_t*)workspace);
     });
 }
 
@@ -62,6 +87,7 @@ namespace {
 int32_t refuse(int32_t code, const char* msg) { gl3_set_create_error(msg); return code; }
 #define OP_ARG(cond, msg) do { if (!(cond)) return refuse(GL3_E_ARG, msg); } while (0)
 
+constexpr int32_t MAX_VOCAB = 1 << 30;
 bool float_type(int32_t t) { return t == GL3_TYPE_F32 || t == GL3_TYPE_F16 || t == GL3_TYPE_BF16; }
 int type_size(int32_t t) { return t == GL3_TYPE_F32 ? 4 : 2; }
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
@@ -165,7 +191,7 @@ int32_t gl3_int8_linear(int32_t device, void* stream, const void* x, int32_t x_t
 
 int32_t gl3_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top, uint64_t* bytes) {
     OP_ARG(bytes, "null pointer");
-    OP_ARG(rows >= 0 && rows <= INT32_MAX && vocab >= 1 && top >= 0 && top <= GL3_LOGPROBS_MAX_TOP, "sizes out of range");
+    OP_ARG(rows >= 0 && rows <= INT32_MAX && vocab >= 1 && vocab <= MAX_VOCAB && top >= 0 && top <= GL3_LOGPROBS_MAX_TOP, "sizes out of range");
     *bytes = rows == 0 ? 0 : op_logprobs_workspace(rows, vocab, top);
     return GL3_OK;
 }
@@ -173,7 +199,7 @@ int32_t gl3_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top, uint64_
 int32_t gl3_token_logprobs(int32_t device, void* stream, const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t ld, const int32_t* targets, int32_t top, float* logprob,
                            int32_t* rank, float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace, uint64_t workspace_bytes) {
     OP_ARG(float_type(type), "logits are GL3_TYPE_F32, F16 or BF16");
-    OP_ARG(rows >= 0 && rows <= INT32_MAX && vocab >= 1, "rows or vocab out of range");
+    OP_ARG(rows >= 0 && rows <= INT32_MAX && vocab >= 1 && vocab <= MAX_VOCAB, "rows or vocab out of range");
     OP_ARG(top >= 0 && top <= GL3_LOGPROBS_MAX_TOP, "top out of range (0 .. GL3_LOGPROBS_MAX_TOP)");
     OP_ARG((targets != nullptr) == (logprob != nullptr) && (targets != nullptr) == (rank != nullptr), "targets, logprob and rank: all or none");
     if (rows == 0) return GL3_OK;

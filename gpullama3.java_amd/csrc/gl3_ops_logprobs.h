@@ -1,88 +1,323 @@
 // gl3_ops_logprobs.h — log probabilities of given tokens, entropy and the most probable tokens of rows of logits (include/gpullama3_hip.h).
+//
+// One pass over the logits.  A wavefront keeps, for what it has seen of a row: the largest logit m (one value, all lanes), per lane
+// s = sum e^(x - m) and t = sum e^(x - m) (x - m) (a new maximum scales both, once per batch of 32 logits a lane at most), how many logits stand
+// in front of the given one, and the best 64 tokens, one a lane, sorted.  A batch touches the list only if one of its logits reaches the smallest
+// of the `top` kept (lo): such logits are collected in LDS, 64 at a time are sorted (bitonic network) and merged.  lo starts as the top-th largest
+// of the first batch's 64 lane maxima, so that batch adds about `top` candidates and not all it holds.
+// With P = sum p (x - m) = t / s:  lse = m + ln s,  logprob = (x_t - m) - ln s,  entropy = ln s - P: both terms >= 0, nothing cancels.
 #pragma once
 #include "gl3_ops_int8.h"          // element types
 
 // A token of a row as one whole number that orders like (logit, lower id first); 0: nothing.  A NaN orders as nothing.
 __device__ __forceinline__ uint64_t op_token_key(float x, int id) {
-    if (!(x > -INFINITY)) return 0;
     const uint32_t b = __float_as_uint(x + 0.f);          // (-0 and +0 are equal logits)
     return (uint64_t)(b >> 31 ? ~b : b | 0x80000000u) << 32 | (uint32_t)~id;
 }
 __device__ __forceinline__ float op_key_logit(uint64_t key) { const uint32_t o = (uint32_t)(key >> 32); return __uint_as_float(o >> 31 ? o & 0x7fffffffu : ~o); }
 __device__ __forceinline__ int op_key_id(uint64_t key) { return (int)~(uint32_t)key; }
-
-// What a part of a row adds to its distribution: s = sum e^(x - m), t = sum e^(x - m) (x - m), over its logits; m its largest.
-struct OpPart { float m, s, t; };
-__device__ __forceinline__ OpPart op_join(const OpPart& a, const OpPart& b) {
-    if (b.s == 0.f) return a;          // (nothing but -inf; a NaN is kept)
-    if (a.s == 0.f) return b;
-    const float m = fmaxf(a.m, b.m), da = a.m - m, db = b.m - m, ea = __expf(da), eb = __expf(db);
-    return OpPart{m, a.s * ea + b.s * eb, (a.t + a.s * da) * ea + (b.t + b.s * db) * eb};
+// the next float32 above x (NaN above +inf and NaN: nothing is)
+__device__ __forceinline__ float op_above(float x) {
+    if (!(x < INFINITY)) return __uint_as_float(0x7fc00000u);
+    if (x == 0.f) return __uint_as_float(1u);
+    const uint32_t b = __float_as_uint(x);
+    return __uint_as_float(b >> 31 ? b - 1 : b + 1);
 }
 
-template <typename T>
-static __global__ __launch_bounds__(256) void op_logprobs_kernel(const T* __restrict__ logits, int vocab, int64_t ld, const int32_t* __restrict__ targets, int top,
-                                                                 float* __restrict__ logprob, int32_t* __restrict__ rank, float* __restrict__ entropy, int32_t* __restrict__ top_ids,
-                                                                 float* __restrict__ top_logprobs) {
-    __shared__ float rm[4], rs[4], rt[4];
-    __shared__ int rc[4], rn[4];
-    __shared__ uint64_t rk[4];
-    const int64_t row = blockIdx.x;
+// ---- lanes ----------------------------------------------------------------------------------------------------------------------------
+template <int M> __device__ __forceinline__ uint32_t op_xor_lane(uint32_t v) {          // the value of lane (lane ^ M)
+    if constexpr (M == 1) return __builtin_amdgcn_mov_dpp((int)v, 0xB1, 0xf, 0xf, true);
+    else if constexpr (M == 2) return __builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);
+    else if constexpr (M == 4) return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true), 0x1B, 0xf, 0xf, true);          // 7 - i, then i ^ 3
+    else if constexpr (M == 8) return __builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true);          // rows of 16, turned by 8
+    else return (uint32_t)__shfl_xor((int)v, M);
+}
+template <int M> __device__ __forceinline__ float op_xor_lane(float v) { return __uint_as_float(op_xor_lane<M>(__float_as_uint(v))); }
+template <int M> __device__ __forceinline__ uint64_t op_xor_lane(uint64_t v) { return (uint64_t)op_xor_lane<M>((uint32_t)(v >> 32)) << 32 | op_xor_lane<M>((uint32_t)v); }
+template <typename V, typename F> __device__ __forceinline__ V op_all_lanes(V v, F f) {
+    v = f(v, op_xor_lane<1>(v)); v = f(v, op_xor_lane<2>(v)); v = f(v, op_xor_lane<4>(v));
+    v = f(v, op_xor_lane<8>(v)); v = f(v, op_xor_lane<16>(v)); return f(v, op_xor_lane<32>(v));
+}
+__device__ __forceinline__ float op_wave_max(float v) { return op_all_lanes(v, [](float a, float b) { return fmaxf(a, b); }); }
+__device__ __forceinline__ float op_wave_sum(float v) { return op_all_lanes(v, [](float a, float b) { return a + b; }); }
+// One step of a bitonic network: lanes `M` apart are exchanged so that the larger value ends in the lane with (lane & M) == 0 where `down`.
+template <int M, typename V> __device__ __forceinline__ V op_exchange(V v, int lane, bool down) {
+    const V o = op_xor_lane<M>(v);
+    return ((o > v) == (((lane & M) == 0) == down)) ? o : v;
+}
+template <int M, typename V> __device__ __forceinline__ V op_clean(V v, int lane, bool down) {          // a bitonic run of 2 M values, sorted
+    v = op_exchange<M>(v, lane, down);
+    if constexpr (M > 1) v = op_clean<M / 2>(v, lane, down);
+    return v;
+}
+template <typename V> __device__ __forceinline__ V op_sort64(V v, int lane) {          // largest in lane 0
+    v = op_clean<1>(v, lane, !(lane & 2)); v = op_clean<2>(v, lane, !(lane & 4)); v = op_clean<4>(v, lane, !(lane & 8));
+    v = op_clean<8>(v, lane, !(lane & 16)); v = op_clean<16>(v, lane, !(lane & 32)); return op_clean<32>(v, lane, true);
+}
+// the 64 largest of two sorted lists of 64
+__device__ __forceinline__ uint64_t op_merge64(uint64_t a, uint64_t b, int lane) {
+    const uint64_t r = (uint64_t)__shfl((unsigned long long)b, 63 - lane);
+    return op_clean<32>(r > a ? r : a, lane, true);
+}
+__device__ __forceinline__ float op_uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
+
+// ---- what a wavefront knows of a row -----------------------------------------------------------------------------------------------------
+constexpr int OP_LP_THREADS = 256, OP_LP_WAVES = OP_LP_THREADS / 64;
+
+struct OpSums { float m, s, t; };          // m = -inf: no logit above -inf so far (s is 0, or NaN)
+__device__ __forceinline__ float op_scale(float from, float to) { return from == -INFINITY ? 1.f : __expf(from - to); }
+__device__ __forceinline__ OpSums op_rescale(OpSums a, float m) {          // to a larger maximum
+    if (a.m == m || a.m == -INFINITY) { a.m = m; return a; }
+    const float d = a.m - m, e = __expf(d);
+    // (d = -inf: nothing of a is left)
+    return OpSums{m, a.s * e, fmaf(a.s, fmaxf(d, -200.f), a.t) * e};
+}
+__device__ __forceinline__ OpSums op_join(const OpSums& a, const OpSums& b) {
+    const float m = fmaxf(a.m, b.m);
+    const OpSums x = op_rescale(a, m), y = op_rescale(b, m);
+    return OpSums{m, x.s + y.s, x.t + y.t};
+}
+
+struct OpTop {
+    uint64_t key;            // the list: lane i holds the i-th best token so far (0: none)
+    float lo;                // a logit below it cannot enter
+    int n;                   // collected candidates
+    bool any;
+    __device__ __forceinline__ void init() { key = 0; lo = -3.402823466e38f; n = 0; any = false; }
+    // 64 of the collected candidates, or what is left of them, into the list
+    __device__ __forceinline__ void merge(uint64_t* buf, int top, int lane) {
+        const int first = max(0, n - 64);
+        const uint64_t c = first + lane < n ? buf[first + lane] : 0;
+        n = first;
+        key = op_merge64(key, op_sort64(c, lane), lane);
+    }
+    // logits behind the ones in the list (higher ids) have to exceed its last one
+    __device__ __forceinline__ void raise(int top, int lane) {
+        const uint32_t hi = __builtin_amdgcn_readlane((uint32_t)(key >> 32), top - 1);
+        if (hi) lo = fmaxf(lo, op_above(op_key_logit((uint64_t)hi << 32)));
+    }
+    __device__ __forceinline__ void collect(uint64_t* buf, float x, int id, bool ok) {
+        const uint64_t pass = __ballot(ok);
+        if (!pass) return;
+        if (ok) buf[n + __popcll(pass & ((1ull << (threadIdx.x & 63)) - 1ull))] = op_token_key(x, id);
+        n += __popcll(pass);
+    }
+};
+
+// One vector of 16 bytes of logits
+template <typename T> struct OpVec { static constexpr int N = 16 / (int)sizeof(T); };
+template <typename T> __device__ __forceinline__ void op_unpack(const uint4& v, float* x) {
+    if constexpr (sizeof(T) == 4) { x[0] = __uint_as_float(v.x); x[1] = __uint_as_float(v.y); x[2] = __uint_as_float(v.z); x[3] = __uint_as_float(v.w); }
+    else {
+        const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            x[2 * i] = op_f32<T>(__builtin_bit_cast(T, (uint16_t)w[i]));
+            x[2 * i + 1] = op_f32<T>(__builtin_bit_cast(T, (uint16_t)(w[i] >> 16)));
+        }
+    }
+}
+
+// What a part of a row leaves for the join: OpPartHead, then `top` keys.
+struct OpPartHead { float m, s, t; int front; };
+static inline __host__ __device__ uint64_t op_part_bytes(int top) { return sizeof(OpPartHead) + 8ull * top; }
+
+struct OpRowOut { const int32_t* targets; int top; float *logprob; int32_t* rank; float* entropy; int32_t* top_ids; float* top_logprobs; };
+
+// One wavefront writes a row's results; k: lane i holds the i-th best token.
+__device__ __forceinline__ void op_row_results(const OpRowOut& o, int64_t row, int vocab, float xt, const OpSums& a, int front, uint64_t k, int lane) {
+    const float nan = __uint_as_float(0x7fc00000u);
+    const bool bad = !(a.s < INFINITY) || a.m == INFINITY, none = !bad && a.m == -INFINITY;
+    const float ls = logf(a.s);
+    auto lp = [&](float v) { return bad ? nan : none ? -INFINITY : (v - a.m) - ls; };
+    if (lane == 0) {
+        if (o.targets) {
+            const int t = o.targets[row];
+            o.logprob[row] = t < 0 ? 0.f : t >= vocab ? nan : lp(xt);
+            o.rank[row] = t < 0 || t >= vocab || xt != xt ? 0 : front + 1;
+        }
+        if (o.entropy) o.entropy[row] = bad ? nan : none ? 0.f : ls - a.t / a.s;
+    }
+    if (lane < o.top) {
+        o.top_ids[row * o.top + lane] = k ? op_key_id(k) : -1;
+        o.top_logprobs[row * o.top + lane] = k ? lp(op_key_logit(k)) : -INFINITY;
+    }
+}
+
+// Grid: x = parts of a row, y = rows (row0 + blockIdx.y).  A part is `per` vectors, a multiple of a workgroup's batch of 256 U; the fewer than
+// 2 x 16 bytes of a row in front of its first whole vector and behind its last one belong to part 0.  parts == 1: the row's results; else a record.
+template <typename T, int U, bool TOP>
+static __global__ __launch_bounds__(OP_LP_THREADS, 4) void op_logprobs_kernel(const T* __restrict__ logits, int vocab, int64_t ld, int64_t row0, int per, OpRowOut o, uint8_t* __restrict__ parts) {
+    constexpr int V = OpVec<T>::N, NT = OP_LP_THREADS;
+    __shared__ uint64_t buf_s[TOP ? OP_LP_WAVES : 1][TOP ? 64 * V + 64 : 1];
+    __shared__ OpSums sums_s[OP_LP_WAVES];
+    __shared__ int front_s[OP_LP_WAVES];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t row = row0 + blockIdx.y;
     const T* x = logits + row * ld;
-    const int t = targets ? targets[row] : -1, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const float xt = t >= 0 && t < vocab ? op_f32<T>(x[t]) : 0.f;
-    float mx = -INFINITY;
-    int bad = 0, front = 0;
-    for (int i = threadIdx.x; i < vocab; i += 256) {
-        const float v = op_f32<T>(x[i]);
-        mx = fmaxf(mx, v);
-        bad |= !(v < INFINITY);
-        front += v > xt || (v == xt && i < t);
+    uint64_t* buf = buf_s[TOP ? wave : 0];
+    const int head = min(vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T)), nv = (vocab - head) / V, tail = vocab - head - nv * V;
+    const uint4* xv = reinterpret_cast<const uint4*>(x + head);
+    const int v0 = blockIdx.x * per, v1 = min(nv, v0 + per);
+    const int t = o.targets ? o.targets[row] : -1;
+    const bool given = t >= 0 && t < vocab;
+    const float nan = __uint_as_float(0x7fc00000u), xt = given ? op_f32<T>(x[t]) : nan, xt_above = op_above(xt);          // (NaN: no logit is counted)
+
+    float m = -INFINITY, s[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
+    int front = 0;
+    OpTop best;
+    best.init();
+    auto batch = [&](int b, auto whole) {          // vectors b + 256 i + thread of the row
+        constexpr bool WHOLE = decltype(whole)::value;
+        float a[U][V];
+        uint4 raw[U];
+        bool in[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int v = b + NT * i + (int)threadIdx.x;
+            in[i] = WHOLE || v < v1;
+            if (in[i]) raw[i] = xv[v];
+        }
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            op_unpack<T>(raw[i], a[i]);
+            if (!WHOLE && !in[i])
+#pragma unroll
+                for (int e = 0; e < V; ++e) a[i][e] = -INFINITY;
+        }
+        float mx = a[0][0];
+#pragma unroll
+        for (int i = 0; i < U; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) mx = fmaxf(mx, a[i][e]);
+        if (__any(mx > m)) {
+            const OpSums n0 = op_rescale(OpSums{m, s[0], u[0]}, op_wave_max(fmaxf(mx, m))), n1 = op_rescale(OpSums{m, s[1], u[1]}, n0.m);
+            s[0] = n0.s; u[0] = n0.t; s[1] = n1.s; u[1] = n1.t;
+            m = op_uniform(n0.m);
+        }
+        const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            const int id = head + (b + NT * i + (int)threadIdx.x) * V;
+            const float th = t >= id + V ? xt : xt_above;          // (the vector that holds t is put right below)
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+                const float d = a[i][e] - ref, p = __expf(d);
+                s[e & 1] += p;
+                u[e & 1] = fmaf(p, fmaxf(d, -200.f), u[e & 1]);          // (0 x -inf stays out; e^-200 is 0)
+                front += __popcll(__ballot(a[i][e] >= th && (WHOLE || in[i])));
+            }
+        }
+        if constexpr (TOP) {
+            if (!best.any) {
+                const uint32_t k = __float_as_uint(mx), ord = k >> 31 ? ~k : k | 0x80000000u, kth = __builtin_amdgcn_readlane(op_sort64(mx == mx ? ord : 0u, lane), o.top - 1);
+                best.lo = fmaxf(best.lo, __uint_as_float(kth >> 31 ? kth & 0x7fffffffu : ~kth));
+                best.any = true;
+            }
+            if (__any(mx >= best.lo)) {
+#pragma unroll 1
+                for (int i = 0; i < U; ++i) {
+                    const int id = head + (b + NT * i + (int)threadIdx.x) * V;
+                    float top1 = a[0][0];
+#pragma unroll
+                    for (int e = 1; e < V; ++e) top1 = fmaxf(top1, a[0][e]);
+                    if (__any(top1 >= best.lo)) {
+#pragma unroll
+                        for (int e = 0; e < V; ++e) best.collect(buf, a[0][e], id + e, a[0][e] >= best.lo);
+                        if (best.n >= 64) {
+                            do best.merge(buf, o.top, lane); while (best.n >= 64);
+                            best.raise(o.top, lane);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j + 1 < U; ++j)          // (registers have no index)
+#pragma unroll
+                        for (int e = 0; e < V; ++e) a[j][e] = a[j + 1][e];
+                }
+            }
+        }
+    };
+    int b = v0;
+    for (; b + NT * U <= v1; b += NT * U) batch(b, std::true_type{});
+    if (b < v1) batch(b, std::false_type{});
+    if (blockIdx.x == 0 && wave == 0) {          // the row's ends, one logit a lane
+        const int id = lane < 32 ? lane : head + nv * V + lane - 32;
+        const bool in = lane < 32 ? lane < head : lane - 32 < tail;
+        const float v = in ? op_f32<T>(x[id]) : -INFINITY;
+        if (__any(v > m)) {
+            const OpSums n0 = op_rescale(OpSums{m, s[0], u[0]}, op_wave_max(fmaxf(v, m))), n1 = op_rescale(OpSums{m, s[1], u[1]}, n0.m);
+            s[0] = n0.s; u[0] = n0.t; s[1] = n1.s; u[1] = n1.t;
+            m = op_uniform(n0.m);
+        }
+        const float d = v - (m == -INFINITY ? 0.f : m), p = __expf(d);
+        s[0] += p;
+        u[0] = fmaf(p, fmaxf(d, -200.f), u[0]);
+        front += __popcll(__ballot(in && (v > xt || (v == xt && id < t))));
+        if constexpr (TOP) {
+            if (best.n) best.merge(buf, o.top, lane);
+            // ids of the head are lower than the list's: equal to its last one is enough
+            best.collect(buf, v, id, in && v > -INFINITY);
+        }
     }
-    for (int d = 32; d; d >>= 1) { mx = fmaxf(mx, __shfl_xor(mx, d)); bad |= __shfl_xor(bad, d); front += __shfl_xor(front, d); }
-    if (lane == 0) { rm[wave] = mx; rc[wave] = bad; rn[wave] = front; }
+    if constexpr (TOP) while (best.n) best.merge(buf, o.top, lane);
+    // logits of t's own vector that stand in front of it with the same value
+    if (given && t >= head && t < head + nv * V && (t - head) / V >= v0 && (t - head) / V < v1 && wave == 0) {
+        const int first = head + (t - head) / V * V;
+        front += __popcll(__ballot(lane < t - first && op_f32<T>(x[first + min(lane, t - first)]) == xt));
+    }
+    const OpSums mine{m, op_wave_sum(s[0] + s[1]), op_wave_sum(u[0] + u[1])};
+    if (lane == 0) { sums_s[wave] = mine; front_s[wave] = front; }
+    if constexpr (TOP) if (wave) buf[lane] = best.key;
     __syncthreads();
-    mx = fmaxf(fmaxf(rm[0], rm[1]), fmaxf(rm[2], rm[3]));
-    bad = rc[0] | rc[1] | rc[2] | rc[3];
-    front = rn[0] + rn[1] + rn[2] + rn[3];
-    float s = 0.f, u = 0.f;
-    if (!bad && mx > -INFINITY)
-        for (int i = threadIdx.x; i < vocab; i += 256) {
-            const float d = op_f32<T>(x[i]) - mx, e = expf(d);
-            s += e;
-            if (e > 0.f) u += e * d;
-        }
-    for (int d = 32; d; d >>= 1) { s += __shfl_xor(s, d); u += __shfl_xor(u, d); }
-    if (lane == 0) { rs[wave] = s; rt[wave] = u; }
-    __syncthreads();
-    s = rs[0] + rs[1] + rs[2] + rs[3];
-    u = rt[0] + rt[1] + rt[2] + rt[3];
-    const bool none = !bad && mx == -INFINITY;
-    const float nan = __uint_as_float(0x7fc00000u), ls = logf(s);
-    auto lp = [&](float v) { return bad ? nan : none ? -INFINITY : (v - mx) - ls; };
-    if (threadIdx.x == 0) {
-        if (targets) {
-            logprob[row] = t < 0 ? 0.f : t >= vocab ? nan : lp(xt);
-            rank[row] = t < 0 || t >= vocab || xt != xt ? 0 : front + 1;
-        }
-        if (entropy) entropy[row] = bad ? nan : none ? 0.f : ls - u / s;
+    if (wave) return;
+    OpSums all = mine;
+#pragma unroll
+    for (int w = 1; w < OP_LP_WAVES; ++w) {
+        all = op_join(all, sums_s[w]);
+        front += front_s[w];
+        if constexpr (TOP) best.key = op_merge64(best.key, buf_s[w][lane], lane);
     }
-    uint64_t last = ~0ull;
-    for (int j = 0; j < top; ++j) {
-        uint64_t best = 0;
-        for (int i = threadIdx.x; i < vocab; i += 256) {
-            const uint64_t key = op_token_key(op_f32<T>(x[i]), i);
-            if (key < last && key > best) best = key;
-        }
-        for (int d = 32; d; d >>= 1) { const uint64_t o = (uint64_t)__shfl_xor((unsigned long long)best, d); best = o > best ? o : best; }
-        __syncthreads();
-        if (lane == 0) rk[wave] = best;
-        __syncthreads();
-        for (int q = 0; q < 4; ++q) best = rk[q] > best ? rk[q] : best;
-        if (threadIdx.x == 0) {
-            top_ids[row * top + j] = best ? op_key_id(best) : -1;
-            top_logprobs[row * top + j] = best ? lp(op_key_logit(best)) : -INFINITY;
-        }
-        last = best;
+    if (gridDim.x == 1) op_row_results(o, row, vocab, xt, all, front, best.key, lane);
+    else {
+        uint8_t* rec = parts + ((uint64_t)row * gridDim.x + blockIdx.x) * op_part_bytes(o.top);
+        if (lane == 0) *reinterpret_cast<OpPartHead*>(rec) = OpPartHead{all.m, all.s, all.t, front};
+        if (TOP && lane < o.top) reinterpret_cast<uint64_t*>(rec + sizeof(OpPartHead))[lane] = best.key;
     }
+}
+
+// The parts of a row (at most 64), joined by one wavefront.
+template <typename T>
+static __global__ __launch_bounds__(64) void op_logprobs_join_kernel(const T* __restrict__ logits, int vocab, int64_t ld, int n, OpRowOut o, const uint8_t* __restrict__ parts) {
+    __shared__ uint64_t buf[128];
+    const int64_t row = blockIdx.x;
+    const int lane = threadIdx.x, top = o.top;
+    const uint64_t bytes = op_part_bytes(top);
+    const uint8_t* rec = parts + (uint64_t)row * n * bytes;
+    const bool in = lane < n;
+    OpPartHead h{-INFINITY, 0.f, 0.f, 0};
+    if (in) h = *reinterpret_cast<const OpPartHead*>(rec + lane * bytes);
+    const float m = op_wave_max(h.m);
+    const OpSums mine = op_rescale(OpSums{h.m, h.s, h.t}, m);
+    const OpSums all{m, op_wave_sum(mine.s), op_wave_sum(mine.t)};
+    const int front = op_all_lanes((uint32_t)h.front, [](uint32_t a, uint32_t b) { return a + b; });
+    OpTop best;
+    best.init();
+    if (top > 0) {
+        // no token behind the best of the parts' last ones is among the first `top`
+        const uint64_t last = in ? reinterpret_cast<const uint64_t*>(rec + lane * bytes + sizeof(OpPartHead))[top - 1] : 0, least = op_all_lanes(last, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
+        for (int i = 0; i < n * top; i += 64) {
+            const int j = i + lane, p = j / top;
+            uint64_t k = 0;
+            if (j < n * top) k = reinterpret_cast<const uint64_t*>(rec + p * bytes + sizeof(OpPartHead))[j - p * top];
+            const bool ok = k != 0 && k >= least;
+            const uint64_t pass = __ballot(ok);
+            if (ok) buf[best.n + __popcll(pass & ((1ull << lane) - 1ull))] = k;
+            best.n += __popcll(pass);
+            if (best.n >= 64) best.merge(buf, top, lane);
+        }
+        if (best.n) best.merge(buf, top, lane);
+    }
+    const int t = o.targets ? o.targets[row] : -1;
+    const float xt = t >= 0 && t < vocab ? op_f32<T>(logits[row * ld + t]) : 0.f;
+    op_row_results(o, row, vocab, xt, all, front, best.key, lane);
 }

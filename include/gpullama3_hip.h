@@ -647,7 +647,8 @@ GL3_API int32_t gl3_int8_workspace(int64_t m, int64_t n, int32_t k, uint64_t* ma
  *   top_ids[r][top], top_logprobs[r][top]   the first `top` tokens of the order (0 <= top <= GL3_LOGPROBS_MAX_TOP); behind the last token of
  *                   non-zero probability (logit above -inf): id -1, -inf.
  * A logit of -inf has probability 0 and adds nothing.  A row of nothing but -inf: log probabilities -inf, entropy 0, no alternatives.  A row that
- * holds a NaN or +inf has NaN log probabilities and entropy; a NaN is never an alternative and no NaN target has a rank (0).  Sums are float32. */
+ * holds a NaN or +inf has NaN log probabilities and entropy; a NaN is never an alternative and no NaN target has a rank (0).  Sums are float32.
+ * 1 <= vocab <= 2^30. */
 #define GL3_LOGPROBS_MAX_TOP 64
 GL3_API int32_t gl3_token_logprobs(int32_t device, void* stream, const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t ld,
                                    const int32_t* targets, int32_t top, float* logprob, int32_t* rank, float* entropy, int32_t* top_ids,
