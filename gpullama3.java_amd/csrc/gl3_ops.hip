@@ -52,7 +52,7 @@ void op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const 
 }
 
 // Parts of a row: as many as give the launch OP_LP_WGS workgroups, none shorter than a small batch, at most 64 (one lane each joins them).
-constexpr int OP_LP_WGS = 1024, OP_LP_SMALL = 2048, OP_LP_BIG = 8192;          // logits of a workgroup's batch
+constexpr int OP_LP_WGS = 1280, OP_LP_SMALL = 2048, OP_LP_BIG = 4096;          // logits of a workgroup's batch
 struct OpLpPlan { int parts, per; bool big; };          // per: logits of a part
 static OpLpPlan op_lp_plan(int64_t rows, int32_t vocab) {
     const int64_t want = std::min<int64_t>(64, std::max<int64_t>(1, OP_LP_WGS / rows));
@@ -78,7 +78,7 @@ void op_logprobs(hipStream_t s, const OpLogprobs& p, void* workspace) {
             else { if (p.top) OP_LP(OP_LP_SMALL / NT / V, true); else OP_LP(OP_LP_SMALL / NT / V, false); }
 #undef OP_LP
         }
-        if (pl.parts > 1) hipLaunchKernelGGL((op_logprobs_join_kernel<T>), dim3((unsigned)p.rows), dim3(64), 0, s, (const T*)p.logits, p.vocab, p.ld, pl.parts, o, (const uint8_t*)workspace);
+        if (pl.parts > 1) hipLaunchKernelGGL((op_logprobs_join_kernel<T>), dim3((unsigned)p.rows), dim3(64 * OP_LP_JOIN_WAVES), 0, s, (const T*)p.logits, p.vocab, p.ld, pl.parts, o, (const uint8_t*)workspace);
     });
 }
 

@@ -30,7 +30,10 @@ template <int M> __device__ __forceinline__ uint32_t op_xor_lane(uint32_t v) {  
     else if constexpr (M == 2) return __builtin_amdgcn_mov_dpp((int)v, 0x4E, 0xf, 0xf, true);
     else if constexpr (M == 4) return __builtin_amdgcn_mov_dpp(__builtin_amdgcn_mov_dpp((int)v, 0x141, 0xf, 0xf, true), 0x1B, 0xf, 0xf, true);          // 7 - i, then i ^ 3
     else if constexpr (M == 8) return __builtin_amdgcn_mov_dpp((int)v, 0x128, 0xf, 0xf, true);          // rows of 16, turned by 8
-    else return (uint32_t)__shfl_xor((int)v, M);
+    else {          // the instruction swaps odd rows (halves) of its first register with even ones of its second: of one value, both neighbours
+        const auto r = [&] { if constexpr (M == 16) return __builtin_amdgcn_permlane16_swap(v, v, false, false); else return __builtin_amdgcn_permlane32_swap(v, v, false, false); }();
+        return threadIdx.x & M ? r[0] : r[1];
+    }
 }
 template <int M> __device__ __forceinline__ float op_xor_lane(float v) { return __uint_as_float(op_xor_lane<M>(__float_as_uint(v))); }
 template <int M> __device__ __forceinline__ uint64_t op_xor_lane(uint64_t v) { return (uint64_t)op_xor_lane<M>((uint32_t)(v >> 32)) << 32 | op_xor_lane<M>((uint32_t)v); }
@@ -40,25 +43,25 @@ template <typename V, typename F> __device__ __forceinline__ V op_all_lanes(V v,
 }
 __device__ __forceinline__ float op_wave_max(float v) { return op_all_lanes(v, [](float a, float b) { return fmaxf(a, b); }); }
 __device__ __forceinline__ float op_wave_sum(float v) { return op_all_lanes(v, [](float a, float b) { return a + b; }); }
-// One step of a bitonic network: lanes `M` apart are exchanged so that the larger value ends in the lane with (lane & M) == 0 where `down`.
-template <int M, typename V> __device__ __forceinline__ V op_exchange(V v, int lane, bool down) {
+// One step of a bitonic network: of two lanes M apart the one with (lane & M) == 0 gets the larger value where DOWN has its bit, else the smaller.
+// Which lane takes what is a constant of the step, so a step is the exchange, one comparison and a select by a mask that the scalar unit makes.
+constexpr uint64_t op_low_lanes(int m) { return m == 1 ? 0x5555555555555555ull : m == 2 ? 0x3333333333333333ull : m == 4 ? 0x0f0f0f0f0f0f0f0full : m == 8 ? 0x00ff00ff00ff00ffull : m == 16 ? 0x0000ffff0000ffffull : m == 32 ? 0x00000000ffffffffull : ~0ull; }
+template <int M, uint64_t DOWN, typename V> __device__ __forceinline__ V op_exchange(V v) {
     const V o = op_xor_lane<M>(v);
-    return ((o > v) == (((lane & M) == 0) == down)) ? o : v;
+    constexpr uint64_t larger = ~(op_low_lanes(M) ^ DOWN);          // lanes that keep the larger value
+    return __builtin_amdgcn_inverse_ballot_w64(~(__builtin_amdgcn_ballot_w64(o > v) ^ larger)) ? o : v;
 }
-template <int M, typename V> __device__ __forceinline__ V op_clean(V v, int lane, bool down) {          // a bitonic run of 2 M values, sorted
-    v = op_exchange<M>(v, lane, down);
-    if constexpr (M > 1) v = op_clean<M / 2>(v, lane, down);
+template <int M, uint64_t DOWN, typename V> __device__ __forceinline__ V op_clean(V v) {          // bitonic runs of 2 M values, sorted
+    v = op_exchange<M, DOWN>(v);
+    if constexpr (M > 1) v = op_clean<M / 2, DOWN>(v);
     return v;
 }
-template <typename V> __device__ __forceinline__ V op_sort64(V v, int lane) {          // largest in lane 0
-    v = op_clean<1>(v, lane, !(lane & 2)); v = op_clean<2>(v, lane, !(lane & 4)); v = op_clean<4>(v, lane, !(lane & 8));
-    v = op_clean<8>(v, lane, !(lane & 16)); v = op_clean<16>(v, lane, !(lane & 32)); return op_clean<32>(v, lane, true);
+template <bool FALLING, typename V> __device__ __forceinline__ V op_sort64(V v) {          // FALLING: largest in lane 0, else in lane 63
+    v = op_clean<1, op_low_lanes(2)>(v); v = op_clean<2, op_low_lanes(4)>(v); v = op_clean<4, op_low_lanes(8)>(v);
+    v = op_clean<8, op_low_lanes(16)>(v); v = op_clean<16, op_low_lanes(32)>(v); return op_clean<32, FALLING ? ~0ull : 0ull>(v);
 }
-// the 64 largest of two sorted lists of 64
-__device__ __forceinline__ uint64_t op_merge64(uint64_t a, uint64_t b, int lane) {
-    const uint64_t r = (uint64_t)__shfl((unsigned long long)b, 63 - lane);
-    return op_clean<32>(r > a ? r : a, lane, true);
-}
+// the 64 largest of two sorted lists of 64, one falling and one rising with the lane
+__device__ __forceinline__ uint64_t op_merge64(uint64_t falling, uint64_t rising) { return op_clean<32, ~0ull>(rising > falling ? rising : falling); }
 __device__ __forceinline__ float op_uniform(float v) { return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v))); }
 
 // ---- what a wavefront knows of a row -----------------------------------------------------------------------------------------------------
@@ -82,14 +85,25 @@ struct OpTop {
     uint64_t key;            // the list: lane i holds the i-th best token so far (0: none)
     float lo;                // a logit below it cannot enter
     int n;                   // collected candidates
-    bool any;
-    __device__ __forceinline__ void init() { key = 0; lo = -3.402823466e38f; n = 0; any = false; }
+    bool any_key;
+    float mine;              // the largest logit this lane has seen
+    int seen, next;          // batches; lo is put up behind batch 1, 2, 4, ...
+    __device__ __forceinline__ void init() { key = 0; lo = -3.402823466e38f; n = 0; any_key = false; mine = -INFINITY; seen = 0; next = 1; }
+    // at least `top` lanes have seen a logit as large as the top-th largest of what the lanes have seen at most: nothing below it can enter
+    __device__ __forceinline__ void batch_max(float mx, int top) {
+        mine = fmaxf(mine, mx);
+        if (++seen < next) return;
+        next = 2 * seen;
+        const uint32_t k = __float_as_uint(mine), kth = __builtin_amdgcn_readlane(op_sort64<true>(k >> 31 ? ~k : k | 0x80000000u), top - 1);
+        lo = fmaxf(lo, __uint_as_float(kth >> 31 ? kth & 0x7fffffffu : ~kth));
+    }
     // 64 of the collected candidates, or what is left of them, into the list
     __device__ __forceinline__ void merge(uint64_t* buf, int top, int lane) {
         const int first = max(0, n - 64);
         const uint64_t c = first + lane < n ? buf[first + lane] : 0;
         n = first;
-        key = op_merge64(key, op_sort64(c, lane), lane);
+        key = any_key ? op_merge64(key, op_sort64<false>(c)) : op_sort64<true>(c);
+        any_key = true;
     }
     // logits behind the ones in the list (higher ids) have to exceed its last one
     __device__ __forceinline__ void raise(int top, int lane) {
@@ -99,6 +113,7 @@ struct OpTop {
     __device__ __forceinline__ void collect(uint64_t* buf, float x, int id, bool ok) {
         const uint64_t pass = __ballot(ok);
         if (!pass) return;
+        asm volatile("" : "+v"(x), "+v"(id));          // (or the keys of all logits are made ahead of the loop around this: 104 instructions a batch)
         if (ok) buf[n + __popcll(pass & ((1ull << (threadIdx.x & 63)) - 1ull))] = op_token_key(x, id);
         n += __popcll(pass);
     }
@@ -147,7 +162,7 @@ __device__ __forceinline__ void op_row_results(const OpRowOut& o, int64_t row, i
 // Grid: x = parts of a row, y = rows (row0 + blockIdx.y).  A part is `per` vectors, a multiple of a workgroup's batch of 256 U; the fewer than
 // 2 x 16 bytes of a row in front of its first whole vector and behind its last one belong to part 0.  parts == 1: the row's results; else a record.
 template <typename T, int U, bool TOP>
-static __global__ __launch_bounds__(OP_LP_THREADS, 4) void op_logprobs_kernel(const T* __restrict__ logits, int vocab, int64_t ld, int64_t row0, int per, OpRowOut o, uint8_t* __restrict__ parts) {
+static __global__ __launch_bounds__(OP_LP_THREADS, 5) void op_logprobs_kernel(const T* __restrict__ logits, int vocab, int64_t ld, int64_t row0, int per, OpRowOut o, uint8_t* __restrict__ parts) {
     constexpr int V = OpVec<T>::N, NT = OP_LP_THREADS;
     __shared__ uint64_t buf_s[TOP ? OP_LP_WAVES : 1][TOP ? 64 * V + 64 : 1];
     __shared__ OpSums sums_s[OP_LP_WAVES];
@@ -167,29 +182,28 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 4) void op_logprobs_kernel(co
     int front = 0;
     OpTop best;
     best.init();
-    auto batch = [&](int b, auto whole) {          // vectors b + 256 i + thread of the row
+    auto load = [&](uint4* raw, int b) {          // vectors b + 256 i + thread of the row (behind the part's end: its last one again)
+#pragma unroll
+        for (int i = 0; i < U; ++i) { const op_v4i q = __builtin_nontemporal_load(reinterpret_cast<const op_v4i*>(xv) + min(b + NT * i + (int)threadIdx.x, v1 - 1)); raw[i] = __builtin_bit_cast(uint4, q); }
+    };
+    auto batch = [&](const uint4* raw, int b, auto whole) {
         constexpr bool WHOLE = decltype(whole)::value;
-        float a[U][V];
-        uint4 raw[U];
+        float a[U][V], vm[U];
         bool in[U];
 #pragma unroll
         for (int i = 0; i < U; ++i) {
-            const int v = b + NT * i + (int)threadIdx.x;
-            in[i] = WHOLE || v < v1;
-            if (in[i]) raw[i] = xv[v];
-        }
-#pragma unroll
-        for (int i = 0; i < U; ++i) {
+            in[i] = WHOLE || b + NT * i + (int)threadIdx.x < v1;
             op_unpack<T>(raw[i], a[i]);
             if (!WHOLE && !in[i])
 #pragma unroll
                 for (int e = 0; e < V; ++e) a[i][e] = -INFINITY;
+            vm[i] = a[i][0];
+#pragma unroll
+            for (int e = 1; e < V; ++e) vm[i] = fmaxf(vm[i], a[i][e]);
         }
-        float mx = a[0][0];
+        float mx = vm[0];
 #pragma unroll
-        for (int i = 0; i < U; ++i)
-#pragma unroll
-            for (int e = 0; e < V; ++e) mx = fmaxf(mx, a[i][e]);
+        for (int i = 1; i < U; ++i) mx = fmaxf(mx, vm[i]);
         if (__any(mx > m)) {
             const OpSums n0 = op_rescale(OpSums{m, s[0], u[0]}, op_wave_max(fmaxf(mx, m))), n1 = op_rescale(OpSums{m, s[1], u[1]}, n0.m);
             s[0] = n0.s; u[0] = n0.t; s[1] = n1.s; u[1] = n1.t;
@@ -202,44 +216,53 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 4) void op_logprobs_kernel(co
             const float th = t >= id + V ? xt : xt_above;          // (the vector that holds t is put right below)
 #pragma unroll
             for (int e = 0; e < V; ++e) {
-                const float d = a[i][e] - ref, p = __expf(d);
+                const float d = a[i][e] - ref, p = __builtin_amdgcn_exp2f(d * 1.44269504f);
                 s[e & 1] += p;
                 u[e & 1] = fmaf(p, fmaxf(d, -200.f), u[e & 1]);          // (0 x -inf stays out; e^-200 is 0)
                 front += __popcll(__ballot(a[i][e] >= th && (WHOLE || in[i])));
             }
         }
         if constexpr (TOP) {
-            if (!best.any) {
-                const uint32_t k = __float_as_uint(mx), ord = k >> 31 ? ~k : k | 0x80000000u, kth = __builtin_amdgcn_readlane(op_sort64(mx == mx ? ord : 0u, lane), o.top - 1);
-                best.lo = fmaxf(best.lo, __uint_as_float(kth >> 31 ? kth & 0x7fffffffu : ~kth));
-                best.any = true;
-            }
-            if (__any(mx >= best.lo)) {
-#pragma unroll 1
-                for (int i = 0; i < U; ++i) {
-                    const int id = head + (b + NT * i + (int)threadIdx.x) * V;
-                    float top1 = a[0][0];
+            best.batch_max(mx, o.top);
+            int i0 = 0;
+            while (i0 < U && __any(mx >= best.lo)) {          // from vector i0 on: until 64 are together
+                int next = U;
 #pragma unroll
-                    for (int e = 1; e < V; ++e) top1 = fmaxf(top1, a[0][e]);
-                    if (__any(top1 >= best.lo)) {
+                for (int i = 0; i < U; ++i)
+                    if (i >= i0 && i < next && __any(vm[i] >= best.lo)) {
+                        const int id = head + (b + NT * i + (int)threadIdx.x) * V;
 #pragma unroll
-                        for (int e = 0; e < V; ++e) best.collect(buf, a[0][e], id + e, a[0][e] >= best.lo);
-                        if (best.n >= 64) {
-                            do best.merge(buf, o.top, lane); while (best.n >= 64);
-                            best.raise(o.top, lane);
-                        }
+                        for (int e = 0; e < V; ++e) best.collect(buf, a[i][e], id + e, a[i][e] >= best.lo);
+                        if (best.n >= 64) next = i + 1;
                     }
-#pragma unroll
-                    for (int j = 0; j + 1 < U; ++j)          // (registers have no index)
-#pragma unroll
-                        for (int e = 0; e < V; ++e) a[j][e] = a[j + 1][e];
+                i0 = next;
+                if (best.n >= 64) {
+                    do best.merge(buf, o.top, lane); while (best.n >= 64);
+                    best.raise(o.top, lane);
                 }
             }
         }
     };
-    int b = v0;
-    for (; b + NT * U <= v1; b += NT * U) batch(b, std::true_type{});
-    if (b < v1) batch(b, std::false_type{});
+    // the next batch is on its way while this one is worked on
+    if (v0 < v1) {
+        uint4 r0[U], r1[U];
+        int b = v0;
+        load(r0, b);
+        for (; b + 2 * NT * U <= v1; b += 2 * NT * U) {
+            load(r1, b + NT * U);
+            batch(r0, b, std::true_type{});
+            if (b + 2 * NT * U < v1) load(r0, b + 2 * NT * U);
+            batch(r1, b + NT * U, std::true_type{});
+        }
+        if (b + NT * U <= v1) {
+            if (b + NT * U < v1) load(r1, b + NT * U);
+            batch(r0, b, std::true_type{});
+            b += NT * U;
+#pragma unroll
+            for (int i = 0; i < U; ++i) r0[i] = r1[i];
+        }
+        if (b < v1) batch(r0, b, std::false_type{});
+    }
     if (blockIdx.x == 0 && wave == 0) {          // the row's ends, one logit a lane
         const int id = lane < 32 ? lane : head + nv * V + lane - 32;
         const bool in = lane < 32 ? lane < head : lane - 32 < tail;
@@ -275,7 +298,7 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 4) void op_logprobs_kernel(co
     for (int w = 1; w < OP_LP_WAVES; ++w) {
         all = op_join(all, sums_s[w]);
         front += front_s[w];
-        if constexpr (TOP) best.key = op_merge64(best.key, buf_s[w][lane], lane);
+        if constexpr (TOP) best.key = op_merge64(best.key, buf_s[w][63 - lane]);
     }
     if (gridDim.x == 1) op_row_results(o, row, vocab, xt, all, front, best.key, lane);
     else {
@@ -285,39 +308,61 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 4) void op_logprobs_kernel(co
     }
 }
 
-// The parts of a row (at most 64), joined by one wavefront.
+// The parts of a row (at most 64), joined by one workgroup: lane i of every wavefront holds part i's sums, wavefront w the lists of parts w, w + 8, ...;
+// all are on their way before the first is looked at (63 parts of 20 tokens one after the other: 18.2 us).
+constexpr int OP_LP_JOIN_WAVES = 8;
 template <typename T>
-static __global__ __launch_bounds__(64) void op_logprobs_join_kernel(const T* __restrict__ logits, int vocab, int64_t ld, int n, OpRowOut o, const uint8_t* __restrict__ parts) {
-    __shared__ uint64_t buf[128];
+static __global__ __launch_bounds__(64 * OP_LP_JOIN_WAVES) void op_logprobs_join_kernel(const T* __restrict__ logits, int vocab, int64_t ld, int n, OpRowOut o, const uint8_t* __restrict__ parts) {
+    constexpr int LISTS = 64 / OP_LP_JOIN_WAVES;
+    __shared__ uint64_t buf[64 * 64];
+    __shared__ int count;
     const int64_t row = blockIdx.x;
-    const int lane = threadIdx.x, top = o.top;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), top = o.top;
     const uint64_t bytes = op_part_bytes(top);
     const uint8_t* rec = parts + (uint64_t)row * n * bytes;
     const bool in = lane < n;
     OpPartHead h{-INFINITY, 0.f, 0.f, 0};
-    if (in) h = *reinterpret_cast<const OpPartHead*>(rec + lane * bytes);
+    uint64_t some = 0, k[LISTS];
+    if (wave == 0 && in) h = *reinterpret_cast<const OpPartHead*>(rec + lane * bytes);
+    const int t = o.targets ? o.targets[row] : -1;
+    const float xt = t >= 0 && t < vocab ? op_f32<T>(logits[row * ld + t]) : 0.f;
+    OpTop best;
+    best.init();
+    if (top > 0) {
+        // q of the parts have j tokens each that are no worse than the q-th best of their j-th ones: with j q >= top nothing below that is among the first `top`
+        const int j = (top + n - 1) / n;
+        if (in) some = reinterpret_cast<const uint64_t*>(rec + lane * bytes + sizeof(OpPartHead))[j - 1];
+#pragma unroll
+        for (int i = 0; i < LISTS; ++i) {
+            const int p = wave + OP_LP_JOIN_WAVES * i;
+            k[i] = p < n && lane < top ? reinterpret_cast<const uint64_t*>(rec + p * bytes + sizeof(OpPartHead))[lane] : 0;
+        }
+        if (threadIdx.x == 0) count = 0;
+        __syncthreads();
+        const int q = (top + j - 1) / j;
+        some = op_sort64<true>(some);
+        const uint64_t least = (uint64_t)__builtin_amdgcn_readlane((uint32_t)(some >> 32), q - 1) << 32 | (uint32_t)__builtin_amdgcn_readlane((uint32_t)some, q - 1);
+#pragma unroll
+        for (int i = 0; i < LISTS; ++i) {
+            const bool ok = k[i] != 0 && k[i] >= least;
+            const uint64_t pass = __ballot(ok);
+            if (pass) {          // (any order: they are sorted)
+                int first = 0;
+                if (lane == 0) first = atomicAdd(&count, (int)__popcll(pass));
+                first = __builtin_amdgcn_readfirstlane(first);
+                if (ok) buf[first + __popcll(pass & ((1ull << lane) - 1ull))] = k[i];
+            }
+        }
+        __syncthreads();
+        if (wave == 0) {
+            best.n = count;
+            while (best.n) best.merge(buf, top, lane);
+        }
+    }
+    if (wave) return;
     const float m = op_wave_max(h.m);
     const OpSums mine = op_rescale(OpSums{h.m, h.s, h.t}, m);
     const OpSums all{m, op_wave_sum(mine.s), op_wave_sum(mine.t)};
     const int front = op_all_lanes((uint32_t)h.front, [](uint32_t a, uint32_t b) { return a + b; });
-    OpTop best;
-    best.init();
-    if (top > 0) {
-        // no token behind the best of the parts' last ones is among the first `top`
-        const uint64_t last = in ? reinterpret_cast<const uint64_t*>(rec + lane * bytes + sizeof(OpPartHead))[top - 1] : 0, least = op_all_lanes(last, [](uint64_t a, uint64_t b) { return a > b ? a : b; });
-        for (int i = 0; i < n * top; i += 64) {
-            const int j = i + lane, p = j / top;
-            uint64_t k = 0;
-            if (j < n * top) k = reinterpret_cast<const uint64_t*>(rec + p * bytes + sizeof(OpPartHead))[j - p * top];
-            const bool ok = k != 0 && k >= least;
-            const uint64_t pass = __ballot(ok);
-            if (ok) buf[best.n + __popcll(pass & ((1ull << lane) - 1ull))] = k;
-            best.n += __popcll(pass);
-            if (best.n >= 64) best.merge(buf, top, lane);
-        }
-        if (best.n) best.merge(buf, top, lane);
-    }
-    const int t = o.targets ? o.targets[row] : -1;
-    const float xt = t >= 0 && t < vocab ? op_f32<T>(logits[row * ld + t]) : 0.f;
     op_row_results(o, row, vocab, xt, all, front, best.key, lane);
 }
