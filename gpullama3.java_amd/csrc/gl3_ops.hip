@@ -26,15 +26,70 @@ void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32
 }
 
 uint64_t op_product_workspace(int64_t, int64_t, int32_t) { return 0; }
+
+template <typename TY, int RT, int MT, int KS, int D>
+static void op_stream_launch(hipStream_t s, const OpProductArgs<TY>& p) {
+    const int64_t strips = op_cdiv(p.n, 16 * RT);
+    const bool once = (int64_t)p.n * p.kp > ((int64_t)128 << 20);
+    const dim3 grid((unsigned)(KS == 1 ? op_cdiv(strips, 4) : strips)), block(64 * (KS == 1 ? 4 : KS));
+    if (once) hipLaunchKernelGGL((op_stream_kernel<TY, RT, MT, KS, D, true>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((op_stream_kernel<TY, RT, MT, KS, D, false>), grid, block, 0, s, p);
+}
+template <typename TY, int MT>
+static void op_stream(hipStream_t s, const OpProductArgs<TY>& p) {
+    if (p.n >= 32768) op_stream_launch<TY, 2, MT, 1, MT == 4 ? 4 : 8>(s, p);
+    else if (p.n >= 8192) op_stream_launch<TY, 2, MT, 4, 4>(s, p);
+    else if (p.n >= 3000) op_stream_launch<TY, 1, MT, 8, 4>(s, p);
+    else op_stream_launch<TY, 1, MT, 16, 4>(s, p);
+}
+template <typename TY, int BM, int BN, int WM, int WN, int SA, int SW>
+static void op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p) {
+    const int mt = (int)op_cdiv(p.m, BM), nt = (int)op_cdiv(p.n, BN);
+    hipLaunchKernelGGL((op_ring_kernel<TY, BM, BN, WM, WN, SA, SW>), dim3((unsigned)op_cdiv((int64_t)mt * nt, 8) * 8), dim3(WM * WN * 64), 0, s, p, mt, nt);
+}
+// Which tile: the one with the least estimated time.  A stage of a BM x BN tile takes a CU 0.00164 (BM + BN) us for its operands' bytes + 0.0000101 BM BN us for its
+// MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 64 x 64 0.25), a tile 3 us and its results' bytes at 20 GB/s besides.  256 CUs take the
+// workgroups in rounds; two workgroups of a small tile share a CU.
+enum { OP_T256x256, OP_T128x256, OP_T256x128, OP_T128x128, OP_T64x128, OP_T64x64, OP_T_COUNT };
+static const struct { int bm, bn, share; } OP_TILES[OP_T_COUNT] = {{256, 256, 1}, {128, 256, 1}, {256, 128, 1}, {128, 128, 2}, {64, 128, 2}, {64, 64, 2}};
+static int op_ring_pick(int m, int n, int kp, int size) {
+    int best = 0;
+    double least = 1e300;
+    for (int t = 0; t < OP_T_COUNT; ++t) {
+        const int bm = OP_TILES[t].bm, bn = OP_TILES[t].bn, slots = 256 * OP_TILES[t].share;
+        const double one = kp / 128 * (0.00164 * (bm + bn) + 0.0000101 * bm * bn) + 3.0 + (double)bm * bn * size / 20e3;
+        const int64_t tiles = op_cdiv(m, bm) * op_cdiv(n, bn), rest = tiles % slots;
+        const double us = (double)(tiles / slots * OP_TILES[t].share + (rest == 0 ? 0 : rest <= 256 ? 1 : 2)) * one;
+        if (us < least) { least = us; best = t; }
+    }
+    return best;
+}
+template <typename TY>
+static void op_ring(hipStream_t s, const OpProductArgs<TY>& p) {
+    switch (op_ring_pick(p.m, p.n, p.kp, sizeof(TY))) {
+        case OP_T256x256: op_ring_launch<TY, 256, 256, 2, 4, 2, 3>(s, p); break;
+        case OP_T128x256: op_ring_launch<TY, 128, 256, 2, 4, 2, 4>(s, p); break;
+        case OP_T256x128: op_ring_launch<TY, 256, 128, 4, 2, 3, 4>(s, p); break;
+        case OP_T128x128: op_ring_launch<TY, 128, 128, 2, 2, 2, 3>(s, p); break;
+        case OP_T64x128: op_ring_launch<TY, 64, 128, 2, 2, 2, 4>(s, p); break;
+        default: op_ring_launch<TY, 64, 64, 2, 2, 4, 5>(s, p);
+    }
+}
+template <typename TY>
+static void op_product_piece(hipStream_t s, const OpProductArgs<TY>& p) {
+    if (p.m <= 16) op_stream<TY, 1>(s, p);
+    else if (p.m <= 32) op_stream<TY, 2>(s, p);
+    else if (p.m <= 64) op_stream<TY, 4>(s, p);
+    else op_ring<TY>(s, p);
+}
 void op_product(hipStream_t s, const OpProduct& p, void*) {
+    constexpr int64_t PM = 1 << 16, PN = 1 << 18;          // a launch's rows and channels: its tiles have 32-bit numbers
     op_with_type(p.y_type, [&](auto t) {
         typedef decltype(t) TY;
-        constexpr int64_t GY = 65535;          // grids of more row tiles go in pieces
-        for (int64_t m0 = 0; m0 < p.m; m0 += GY * 16) {
-            const int64_t m = std::min(p.m - m0, GY * 16);
-            hipLaunchKernelGGL((op_product_kernel<TY>), dim3((unsigned)op_cdiv(p.n, 16), (unsigned)op_cdiv(m, 16)), dim3(64), 0, s, p.a + m0 * p.lda, p.lda, p.a_scale + m0, p.w, p.ldw,
-                               p.w_scale, p.bias, m, p.n, p.k, (TY*)p.y + m0 * p.ldy, p.ldy);
-        }
+        for (int64_t n = 0; n < p.n; n += PN)
+            for (int64_t m = 0; m < p.m; m += PM)
+                op_product_piece(s, OpProductArgs<TY>{p.a + m * p.lda, p.lda, p.a_scale + m, p.w + n * p.ldw, p.ldw, p.w_scale + n, p.bias ? p.bias + n : nullptr, (int)std::min(PM, p.m - m),
+                                                      (int)std::min(PN, p.n - n), (int)op_code_ld(p.k), (TY*)p.y + m * p.ldy + n, p.ldy});
     });
 }
 
@@ -92,6 +147,8 @@ bool float_type(int32_t t) { return t == GL3_TYPE_F32 || t == GL3_TYPE_F16 || t 
 int type_size(int32_t t) { return t == GL3_TYPE_F32 ? 4 : 2; }
 bool aligned(const void* p, size_t to) { return ((uintptr_t)p & (to - 1)) == 0; }
 // rows of `cols` elements, `ld` apart (one row: any ld): whether their bytes fit an address
+constexpr int64_t MAX_Y_LD = 1 << 26;
+constexpr int64_t MAX_CODE_LD = 1 << 23;          // (a tile's rows are reached with 32-bit offsets)
 bool rows_ok(int64_t rows, int64_t cols, int64_t ld) { return rows <= 1 || (ld >= cols && ld <= (INT64_MAX >> 4) / rows); }
 
 // the caller's device for the length of a call
@@ -121,9 +178,9 @@ int32_t check_product(const OpProduct& p) {
     if (p.m == 0 || p.n == 0) return GL3_OK;
     OP_ARG(p.w && p.w_scale && p.y, "null pointer");
     OP_ARG(aligned(p.w, 16) && p.ldw % 16 == 0, "codes start on 16 bytes, and so does every row of them");
-    OP_ARG(rows_ok(p.n, op_code_ld(p.k), p.ldw), "ldw: a row of codes is k columns and zeros up to a multiple of GL3_CODE_BLOCK");
+    OP_ARG(rows_ok(p.n, op_code_ld(p.k), p.ldw) && p.ldw <= MAX_CODE_LD, "ldw: a row of codes is k columns and zeros up to a multiple of GL3_CODE_BLOCK");
     OP_ARG(aligned(p.w_scale, 4) && aligned(p.bias, 4) && aligned(p.y, type_size(p.y_type)), "misaligned pointer");
-    OP_ARG(rows_ok(p.m, p.n, p.ldy), "ldy is less than n");
+    OP_ARG(rows_ok(p.m, p.n, p.ldy) && (p.m <= 1 || p.ldy <= MAX_Y_LD), "ldy out of range (n .. 2^26)");
     return GL3_OK;
 }
 int32_t check_workspace(const void* workspace, uint64_t have, uint64_t need) {
@@ -166,7 +223,7 @@ int32_t gl3_int8_matmul(int32_t device, void* stream, const int8_t* a, int64_t l
     if (r != GL3_OK || m == 0 || n == 0) return r;
     OP_ARG(a && a_scale, "null pointer");
     OP_ARG(aligned(a, 16) && lda % 16 == 0, "codes start on 16 bytes, and so does every row of them");
-    OP_ARG(rows_ok(m, op_code_ld(k), lda) && aligned(a_scale, 4), "lda: a row of codes is k columns and zeros up to a multiple of GL3_CODE_BLOCK");
+    OP_ARG(rows_ok(m, op_code_ld(k), lda) && lda <= MAX_CODE_LD && aligned(a_scale, 4), "lda: a row of codes is k columns and zeros up to a multiple of GL3_CODE_BLOCK");
     if ((r = check_workspace(workspace, workspace_bytes, op_product_workspace(m, n, k))) != GL3_OK) return r;
     OnDevice on;
     if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);

@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 typedef int op_v4i __attribute__((ext_vector_type(4)));
 typedef int op_v16i __attribute__((ext_vector_type(16)));
@@ -54,26 +55,259 @@ static __global__ __launch_bounds__(256) void op_quantize_kernel(const T* __rest
 
 // ---- products -------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float op_result(int acc, float as, float ws) { return ((float)acc * as) * ws; }
+template <bool ONCE> __device__ __forceinline__ op_v4i op_load16(const int8_t* p) {
+    const op_v4i* q = reinterpret_cast<const op_v4i*>(p);
+    return ONCE ? __builtin_nontemporal_load(q) : *q;
+}
+template <typename TY> struct OpProductArgs {
+    const int8_t* a; int64_t lda; const float* as;
+    const int8_t* w; int64_t ldw; const float* ws; const float* bias;
+    int m, n, kp;            // kp: k rounded up to a multiple of 128
+    TY* y; int64_t ldy;
+};
 
-// One wavefront per 16 tokens x 16 channels, both operands straight from memory: a lane holds 16 consecutive k of one row of either.
-template <typename TY>
-static __global__ __launch_bounds__(64) void op_product_kernel(const int8_t* __restrict__ a, int64_t lda, const float* __restrict__ as, const int8_t* __restrict__ w, int64_t ldw,
-                                                               const float* __restrict__ ws, const float* __restrict__ bias, int64_t m, int64_t n, int k, TY* __restrict__ y, int64_t ldy) {
-    const int lane = threadIdx.x, r16 = lane & 15, kg = lane >> 4;
-    const int64_t n0 = (int64_t)blockIdx.x * 16, m0 = (int64_t)blockIdx.y * 16;
-    const int8_t* ap = a + min(m0 + r16, m - 1) * lda + 16 * kg;
-    const int8_t* wp = w + min(n0 + r16, n - 1) * ldw + 16 * kg;
-    op_v4i acc = {0, 0, 0, 0};
-    for (int c = 0; c < k; c += 64)          // (rows end on a multiple of 128)
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(*reinterpret_cast<const op_v4i*>(ap + c), *reinterpret_cast<const op_v4i*>(wp + c), acc, 0, 0, 0);
-    const int64_t col = n0 + r16;
-    if (col >= n) return;
-    const float sw = ws[col], b = bias ? bias[col] : 0.f;
+// Up to 64 tokens: the weights' bytes are what it costs, and they go from memory to the matrix cores' registers directly.  A wavefront has 16 RT
+// channels x 16 MT tokens (v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l % 16) and a ring of D steps of 64 k on their way; the
+// tokens' codes come from the caches.  KS wavefronts of a workgroup share the channels and split k (their int32 sums meet in LDS: exact in any
+// order); KS = 1: four wavefronts with channels of their own.
+template <typename TY, int RT, int MT, int KS, int D, bool ONCE>
+static __global__ __launch_bounds__(64 * (KS == 1 ? 4 : KS)) void op_stream_kernel(OpProductArgs<TY> p) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kg = lane >> 4;
+    const int n0 = (KS == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x) * 16 * RT;
+    if (KS == 1 && n0 >= p.n) return;
+    const int steps = p.kp / 64, s0 = KS == 1 ? 0 : (int)((int64_t)steps * wave / KS), cnt = (KS == 1 ? steps : (int)((int64_t)steps * (wave + 1) / KS)) - s0;
+    const int8_t *wb = p.w + (int64_t)n0 * p.ldw + (int64_t)s0 * 64, *ab = p.a + (int64_t)s0 * 64;          // (uniform; the lanes' parts fit 32 bits)
+    uint32_t wo[RT], ao[MT];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int64_t row = m0 + 4 * kg + r;
-        if (row >= m) break;
-        const float v = op_result(acc[r], as[row], sw);
-        y[row * ldy + col] = op_cast<TY>(bias ? v + b : v);
+    for (int i = 0; i < RT; ++i) wo[i] = (uint32_t)(min(n0 + 16 * i + r16, p.n - 1) - n0) * (uint32_t)p.ldw + 16 * kg;          // (rows past the end repeat the last one)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) ao[j] = (uint32_t)min(16 * j + r16, p.m - 1) * (uint32_t)p.lda + 16 * kg;
+    op_v4i acc[RT][MT], fw[D][RT], fa[D][MT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) acc[i][j] = op_v4i{0, 0, 0, 0};
+    auto load = [&](int d, int s) {
+        const int8_t *w = wb + (int64_t)s * 64, *a = ab + (int64_t)s * 64;
+#pragma unroll
+        for (int i = 0; i < RT; ++i) fw[d][i] = op_load16<ONCE>(w + wo[i]);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) fa[d][j] = op_load16<false>(a + ao[j]);
+    };
+    auto mma = [&](int d) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[d][i], fa[d][j], acc[i][j], 0, 0, 0);
+    };
+    if (cnt > 0) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) load(d, min(d, cnt - 1));
+        int s = 0;
+        for (; s + D < cnt; s += D)
+#pragma unroll
+            for (int d = 0; d < D; ++d) { mma(d); load(d, min(s + D + d, cnt - 1)); }
+#pragma unroll
+        for (int d = 0; d < D; ++d) if (s + d < cnt) mma(d);
     }
+    auto store = [&](const op_v4i& v, int i, int j) {          // lane: token l % 16, channels 4 (l / 16) ..
+        const int row = 16 * j + r16, col = n0 + 16 * i + 4 * kg;
+        if (row >= p.m) return;
+        const float sa = p.as[row];
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (col + r < p.n) {
+                const float x = op_result(v[r], sa, p.ws[col + r]);
+                p.y[(int64_t)row * p.ldy + col + r] = op_cast<TY>(p.bias ? x + p.bias[col + r] : x);
+            }
+    };
+    if constexpr (KS == 1) {
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) store(acc[i][j], i, j);
+    } else {
+        __shared__ op_v4i part[KS][RT * MT][64];
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int j = 0; j < MT; ++j) part[wave][i * MT + j][lane] = acc[i][j];
+        __syncthreads();
+        for (int t = wave; t < RT * MT; t += KS) {
+            op_v4i v = part[0][t][lane];
+#pragma unroll
+            for (int q = 1; q < KS; ++q) v += part[q][t][lane];
+            store(v, t / MT, t % MT);
+        }
+    }
+}
+
+// More tokens: BM tokens x BN channels per workgroup of WM x WN wavefronts, v_mfma_i32_32x32x32_i8.  The operands go straight to LDS (16 bytes a lane, no
+// registers in between) into rings of SA stages of a and SW of w, a stage being 128 k of every row; the barrier of a stage stands in front of its last
+// quarter, so the matrix cores have that quarter while the next stage's first fragments are read, and it waits for all loads but those that have a
+// stage left to travel.  16-byte chunk c of row r stands at chunk c ^ (r / 2 % 8): the 16 lanes of a read cover the banks once.  Workgroups go to the
+// 8 XCDs in turn; the token tiles of one channel tile run on one XCD, so its weights leave HBM once.
+__device__ __forceinline__ void op_dma16(const void* src, void* lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
+}
+// all but the newest N loads of this wavefront have landed, its LDS reads are done, and so are everybody's
+template <int I, int N, typename F> __device__ __forceinline__ void op_static_for(F f) { if constexpr (I < N) { f(std::integral_constant<int, I>{}); op_static_for<I + 1, N>(f); } }
+template <int N> __device__ __forceinline__ void op_wait_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory"); }
+
+template <typename TY, int BM, int BN, int WM, int WN, int SA, int SW>
+static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProductArgs<TY> p, int mt, int nt) {
+    constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+    constexpr int PA = BM / 8, PW = BN / 8, NPA = (PA + NW - 1) / NW, NPW = (PW + NW - 1) / NW, NP = NPA + NPW;          // 1 KB pieces (8 rows) of a stage, per wavefront
+    constexpr int SZA = BM * 128, SZW = BN * 128, OW = SA * SZA;
+    static_assert(SW >= SA + 1 && SA >= 2 && TM * WM * 32 == BM && TN * WN * 32 == BN, "tile layout");
+    static_assert(SA * SZA + SW * SZW <= 160 * 1024 && BM <= NW * 64 && BN <= NW * 64, "LDS; a scale per thread");
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[SA * SZA + SW * SZW];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
+    const int total = mt * nt, per_xcd = (total + 7) >> 3, J = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
+    if (J >= total) return;
+    const int m0 = (J % mt) * BM, n0 = (J / mt) * BN, n_it = p.kp / 128;
+    const int8_t *ab = p.a + m0 * p.lda, *wb = p.w + n0 * p.ldw;
+    // this wavefront's pieces (rows past the end repeat the last one: their results are not stored; wavefronts without a piece of their own load one again)
+    uint32_t offa[NPA], offw[NPW];
+    int pa[NPA], pw[NPW];
+#pragma unroll
+    for (int u = 0; u < NPA; ++u) {
+        const int q = (wave + NW * u) % PA, row = 8 * q + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+        pa[u] = q * 1024;
+        offa[u] = (uint32_t)(min(m0 + row, p.m - 1) - m0) * (uint32_t)p.lda + 16 * c;
+    }
+#pragma unroll
+    for (int u = 0; u < NPW; ++u) {
+        const int q = (wave + NW * u) % PW, row = 8 * q + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
+        pw[u] = OW + q * 1024;
+        offw[u] = (uint32_t)(min(n0 + row, p.n - 1) - n0) * (uint32_t)p.ldw + 16 * c;
+    }
+    // scales of the tile's rows and columns, one a thread: needed at the end, in LDS
+    const int my_m = min(m0 + (tid < BM ? tid : 0), p.m - 1), my_n = min(n0 + (tid < BN ? tid : 0), p.n - 1);
+    const float my_as = p.as[my_m], my_ws = p.ws[my_n], my_b = p.bias ? p.bias[my_n] : 0.f;
+    constexpr int WH = (NPW + 1) / 2;
+    auto issue_a = [&](int it, int slot) {
+        const int8_t* a = ab + (int64_t)it * 128;
+#pragma unroll
+        for (int u = 0; u < NPA; ++u) op_dma16(a + offa[u], smem + slot * SZA + pa[u]);
+    };
+    auto issue_w = [&](int it, int slot, int u0, int u1) {
+        const int8_t* w = wb + (int64_t)it * 128;
+#pragma unroll
+        for (int u = 0; u < NPW; ++u)
+            if (u >= u0 && u < u1) op_dma16(w + offw[u], smem + slot * SZW + pw[u]);
+    };
+    op_v16i acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0;
+    const int r32 = lane & 31, kh = lane >> 5;
+    uint32_t ca[4];          // a stage is four quarters of 32 k: a lane reads row lane % 32, chunk 2 quarter + lane / 32
+#pragma unroll
+    for (int q = 0; q < 4; ++q) ca[q] = ((2 * q + kh) ^ ((r32 >> 1) & 7)) * 16;
+    const uint32_t aw = (wm * (BM / WM) + r32) * 128, ww = OW + (wn * (BN / WN) + r32) * 128;
+    // step s (behind barrier s) starts the loads of a's stage s + SA (into the slot the barrier freed) and, in the two quarters after it, of w's stage
+    // s + SW; the steps before 0 are the prologue, the last one's w belongs to the loop's first round
+    constexpr int LEFT = (SA - 2) * NP + NPW;          // loads started behind a's stage s + 1 when barrier s waits for it
+#pragma unroll
+    for (int s = -SW; s < 0; ++s) {
+        if (s + SA >= 0 && s + SA < n_it) issue_a(s + SA, s + SA);
+        if (s < -1 && s + SW < n_it) issue_w(s + SW, s + SW, 0, NPW);
+    }
+    if (n_it >= SW) op_wait_barrier<(SA - 1) * NP>(); else op_wait_barrier<0>();
+    int sa = 0, sw = 0, sp = SW - 1, it = 0;          // slots of the current stage; sp: the w slot that the step before fills
+    op_v4i fa[2][TM], fw[2][TN];
+    constexpr int NR = TM + TN, NM = TM * TN;
+    auto rd1 = [&](int set, int q, int f) {          // fragment f of a quarter: TM of a, TN of w
+        if (f < TM) fa[set][f] = *reinterpret_cast<const op_v4i*>(smem + sa * SZA + aw + f * 4096 + ca[q]);
+        else fw[set][f - TM] = *reinterpret_cast<const op_v4i*>(smem + sw * SZW + ww + (f - TM) * 4096 + ca[q]);
+    };
+    // A quarter: its MFMAs with the next quarter's fragment reads (RPM behind each of the first ones) and then ND loads between them, in this very order
+    // (all reads have to stand in front of the loads: both are in LDS, and nobody tells the compiler that they are apart).  The reads are waited for at its
+    // end, where the compiler sees it (else it waits in front of the next quarter's first MFMA for a read that has just been started as well).
+    constexpr int RPM = 2, NRM = (NR + RPM - 1) / RPM;
+    auto quarter = [&](auto set_, auto q_, bool more, auto nd_, auto load) {
+        constexpr int set = decltype(set_)::value, q = decltype(q_)::value, ND = decltype(nd_)::value, ROOM = NM > NRM ? NM - NRM : 1;
+        op_static_for<0, NM>([&](auto c_) {
+            constexpr int c = decltype(c_)::value;
+            acc[c / TN][c % TN] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[set][c / TN], fw[set][c % TN], acc[c / TN][c % TN], 0, 0, 0);
+            if constexpr (c < NRM || c == NM - 1) {
+                if (more)
+                    op_static_for<0, (c == NM - 1 && c < NRM ? NR : RPM)>([&](auto f) { constexpr int fr = c * RPM + decltype(f)::value; if constexpr (fr < NR) rd1(1 - set, q, fr); });
+            }
+            if constexpr (NM <= NRM) { if constexpr (c == NM - 1) op_static_for<0, ND>([&](auto u) { load(u); }); }
+            else if constexpr (c >= NRM) op_static_for<(c - NRM) * ND / ROOM, (c - NRM + 1) * ND / ROOM>([&](auto u) { load(u); });
+            __builtin_amdgcn_sched_barrier(0);
+        });
+        __builtin_amdgcn_s_waitcnt(0xc07f);
+    };
+    constexpr std::integral_constant<int, 0> I0{};
+    constexpr std::integral_constant<int, 1> I1{};
+    constexpr std::integral_constant<int, 2> I2{};
+    constexpr std::integral_constant<int, 3> I3{};
+    constexpr std::integral_constant<int, WH> IW0{};
+    constexpr std::integral_constant<int, NPW - WH> IW1{};
+    constexpr std::integral_constant<int, NPA> IA{};
+    auto nothing = [](auto) {};
+    op_static_for<0, NR>([&](auto f) { rd1(0, 0, decltype(f)::value); });
+    __builtin_amdgcn_s_waitcnt(0xc07f);
+    for (; it < n_it - SW; ++it) {
+        const int8_t* gw = wb + (int64_t)(it - 1 + SW) * 128;
+        uint8_t* dw = smem + sp * SZW;
+        quarter(I0, I1, true, IW0, [&](auto u) { constexpr int v = decltype(u)::value; op_dma16(gw + offw[v], dw + pw[v]); });
+        quarter(I1, I2, true, IW1, [&](auto u) { constexpr int v = WH + decltype(u)::value; op_dma16(gw + offw[v], dw + pw[v]); });
+        quarter(I0, I3, true, I0, nothing);
+        op_wait_barrier<LEFT>();
+        const int8_t* ga = ab + (int64_t)(it + SA) * 128;
+        uint8_t* da = smem + sa * SZA;
+        sp = sw;
+        if (++sa == SA) sa = 0;
+        if (++sw == SW) sw = 0;
+        quarter(I1, I0, true, IA, [&](auto u) { constexpr int v = decltype(u)::value; op_dma16(ga + offa[v], da + pa[v]); });
+    }
+    if (it - 1 + SW < n_it) issue_w(it - 1 + SW, sp, 0, NPW);
+    for (; it < n_it; ++it) {          // the last SW stages: nothing (a: little) left to load
+        quarter(I0, I1, true, I0, nothing);
+        quarter(I1, I2, true, I0, nothing);
+        quarter(I0, I3, true, I0, nothing);
+        op_wait_barrier<0>();
+        if (it + SA < n_it) issue_a(it + SA, sa);
+        if (++sa == SA) sa = 0;
+        if (++sw == SW) sw = 0;
+        quarter(I1, I0, it + 1 < n_it, I0, nothing);
+    }
+    // Lane holds channel lane % 32 and tokens 8 (r / 4) + 4 (lane / 32) + r % 4 of every 32 x 32 tile.  A store's row comes from the scalar unit, the lane's
+    // part is one 32-bit offset.  (Behind the last barrier nobody reads the rings and no load is on its way.)
+    float *las = reinterpret_cast<float*>(smem), *lws = las + BM, *lb = lws + BN;
+    if (tid < BM) las[tid] = my_as;
+    if (tid < BN) { lws[tid] = my_ws; lb[tid] = my_b; }
+    __syncthreads();
+    const int mb = m0 + wm * (BM / WM), nb = n0 + wn * (BN / WN);
+    const bool whole = m0 + BM <= p.m && n0 + BN <= p.n, biased = p.bias != nullptr;
+    const uint32_t lo = ((uint32_t)(4 * kh) * (uint32_t)p.ldy + r32) * (uint32_t)sizeof(TY);
+    auto store = [&](auto all) {
+        constexpr bool ALL = decltype(all)::value;
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int cn = wn * (BN / WN) + j * 32 + r32;
+            const float w_ = lws[cn], b_ = lb[cn];
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float* s4 = las + wm * (BM / WM) + i * 32 + 8 * g + 4 * kh;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int row = mb + i * 32 + 8 * g + r;          // (of lanes 0 .. 31)
+                        const float x = op_result(acc[i][j][4 * g + r], s4[r], w_);
+                        if (ALL || (row + 4 * kh < p.m && n0 + cn < p.n))
+                            *reinterpret_cast<TY*>(reinterpret_cast<uint8_t*>(p.y + row * p.ldy + nb + j * 32) + lo) = op_cast<TY>(biased ? x + b_ : x);
+                    }
+                }
+        }
+    };
+    if (whole) store(std::true_type{}); else store(std::false_type{});
 }

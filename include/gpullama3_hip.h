@@ -628,7 +628,7 @@ GL3_API int32_t gl3_quantize_rows(int32_t device, void* stream, const void* x, i
                                   int8_t* codes, int64_t ldq, float* scale);
 /* y[i][j] = (float(sum_k a[i][k] w[j][k]) * a_scale[i]) * w_scale[j] (+ bias[j]): m rows of codes against n channels of codes, both as
  * gl3_quantize_rows lays them out (16-byte aligned, strides multiples of 16, zeros from column k to the next multiple of GL3_CODE_BLOCK); the sum
- * is exact in int32, whatever the codes (k <= GL3_INT8_MAX_K).  bias: float32 or NULL.  y: GL3_TYPE_F32 / F16 / BF16, one rounding.  m, n < 2^31. */
+ * is exact in int32, whatever the codes (k <= GL3_INT8_MAX_K).  lda, ldw <= 2^23, ldy <= 2^26.  bias: float32 or NULL.  y: GL3_TYPE_F32 / F16 / BF16, one rounding.  m, n < 2^31. */
 GL3_API int32_t gl3_int8_matmul(int32_t device, void* stream, const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw,
                                 const float* w_scale, const float* bias, int64_t m, int64_t n, int32_t k, void* y, int32_t y_type, int64_t ldy,
                                 void* workspace, uint64_t workspace_bytes);
