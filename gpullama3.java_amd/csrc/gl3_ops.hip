@@ -20,39 +20,29 @@ template <typename F> static void op_with_type(int32_t type, F&& f) {
 void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale) {
     op_with_type(type, [&](auto t) {
         typedef decltype(t) T;
-        for (int64_t r = 0; r < rows; r += OP_GRID)
-            hipLaunchKernelGGL((op_quantize_kernel<T>), dim3((unsigned)std::min<int64_t>(OP_GRID, rows - r)), dim3(256), 0, s, (const T*)x + r * ldx, cols, ldx, codes + r * ldq, ldq, scale + r);
+        const int64_t kp = op_code_ld(cols);
+        for (int64_t r = 0; r < rows; r += OP_GRID) {
+            const int64_t n = std::min<int64_t>(OP_GRID, rows - r);
+            const T* xr = (const T*)x + r * ldx;
+#define OP_Q(W) hipLaunchKernelGGL((op_quantize_kernel<T, W>), dim3((unsigned)(W > 4 ? n : op_cdiv(n * W, 4))), dim3(W > 4 ? 64 * W : 256), 0, s, xr, n, cols, ldx, codes + r * ldq, ldq, scale + r)
+            // as many wavefronts a row as it needs; of a few rows more, so that a thread has 16 bytes or so
+            if (kp <= 512 || (kp <= OP_ROW_E * 64 && rows > 2048)) OP_Q(1);
+            else if (kp <= OP_ROW_E * 256 && (kp <= 2048 || rows > 64)) OP_Q(4);
+            else if (kp <= OP_ROW_E * 1024) OP_Q(16);
+            else hipLaunchKernelGGL((op_quantize_long_kernel<T>), dim3((unsigned)n), dim3(1024), 0, s, xr, cols, ldx, codes + r * ldq, ldq, scale + r);
+#undef OP_Q
+        }
     });
 }
 
 uint64_t op_product_workspace(int64_t, int64_t, int32_t) { return 0; }
 
-template <typename TY, int RT, int MT, int KS, int D>
-static void op_stream_launch(hipStream_t s, const OpProductArgs<TY>& p) {
-    const int64_t strips = op_cdiv(p.n, 16 * RT);
-    const bool once = (int64_t)p.n * p.kp > ((int64_t)128 << 20);
-    const dim3 grid((unsigned)(KS == 1 ? op_cdiv(strips, 4) : strips)), block(64 * (KS == 1 ? 4 : KS));
-    if (once) hipLaunchKernelGGL((op_stream_kernel<TY, RT, MT, KS, D, true>), grid, block, 0, s, p);
-    else hipLaunchKernelGGL((op_stream_kernel<TY, RT, MT, KS, D, false>), grid, block, 0, s, p);
-}
-template <typename TY, int MT>
-static void op_stream(hipStream_t s, const OpProductArgs<TY>& p) {
-    if (p.n >= 32768) op_stream_launch<TY, 2, MT, 1, MT == 4 ? 4 : 8>(s, p);
-    else if (p.n >= 8192) op_stream_launch<TY, 2, MT, 4, 4>(s, p);
-    else if (p.n >= 3000) op_stream_launch<TY, 1, MT, 8, 4>(s, p);
-    else op_stream_launch<TY, 1, MT, 16, 4>(s, p);
-}
-template <typename TY, int BM, int BN, int WM, int WN, int SA, int SW>
-static void op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p) {
-    const int mt = (int)op_cdiv(p.m, BM), nt = (int)op_cdiv(p.n, BN);
-    hipLaunchKernelGGL((op_ring_kernel<TY, BM, BN, WM, WN, SA, SW>), dim3((unsigned)op_cdiv((int64_t)mt * nt, 8) * 8), dim3(WM * WN * 64), 0, s, p, mt, nt);
-}
 // Which tile: the one with the least estimated time.  A stage of a BM x BN tile takes a CU 0.00164 (BM + BN) us for its operands' bytes + 0.0000101 BM BN us for its
 // MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 64 x 64 0.25), a tile 3 us and its results' bytes at 20 GB/s besides.  256 CUs take the
 // workgroups in rounds; two workgroups of a small tile share a CU.
 enum { OP_T256x256, OP_T128x256, OP_T256x128, OP_T128x128, OP_T64x128, OP_T64x64, OP_T_COUNT };
 static const struct { int bm, bn, share; } OP_TILES[OP_T_COUNT] = {{256, 256, 1}, {128, 256, 1}, {256, 128, 1}, {128, 128, 2}, {64, 128, 2}, {64, 64, 2}};
-static int op_ring_pick(int m, int n, int kp, int size) {
+static int op_ring_pick(int m, int n, int kp, int size, double* us_out) {
     int best = 0;
     double least = 1e300;
     for (int t = 0; t < OP_T_COUNT; ++t) {
@@ -62,11 +52,17 @@ static int op_ring_pick(int m, int n, int kp, int size) {
         const double us = (double)(tiles / slots * OP_TILES[t].share + (rest == 0 ? 0 : rest <= 256 ? 1 : 2)) * one;
         if (us < least) { least = us; best = t; }
     }
+    *us_out = std::max(least, (double)n * kp / 5.4e6 + 4.0);          // the weights leave memory at 5.4 TB/s
     return best;
 }
+template <typename TY, int BM, int BN, int WM, int WN, int SA, int SW>
+static void op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p) {
+    const int mt = (int)op_cdiv(p.m, BM), nt = (int)op_cdiv(p.n, BN);
+    hipLaunchKernelGGL((op_ring_kernel<TY, BM, BN, WM, WN, SA, SW>), dim3((unsigned)op_cdiv((int64_t)mt * nt, 8) * 8), dim3(WM * WN * 64), 0, s, p, mt, nt);
+}
 template <typename TY>
-static void op_ring(hipStream_t s, const OpProductArgs<TY>& p) {
-    switch (op_ring_pick(p.m, p.n, p.kp, sizeof(TY))) {
+static void op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile) {
+    switch (tile) {
         case OP_T256x256: op_ring_launch<TY, 256, 256, 2, 4, 2, 3>(s, p); break;
         case OP_T128x256: op_ring_launch<TY, 128, 256, 2, 4, 2, 4>(s, p); break;
         case OP_T256x128: op_ring_launch<TY, 256, 128, 4, 2, 3, 4>(s, p); break;
@@ -75,12 +71,20 @@ static void op_ring(hipStream_t s, const OpProductArgs<TY>& p) {
         default: op_ring_launch<TY, 64, 64, 2, 2, 4, 5>(s, p);
     }
 }
+// Up to 32 tokens may be streamed: 6.6 TB/s of weights, 4.2 % more time a token (us, streamed / tiles; m tokens, n x k: 1, 4096 x 4096 6.5 / 10.3; 16 8.0 / 10.8;
+// 32 9.6 / 11.3; 16, 4096 x 14336 17.7 / 25.2; 4, 14336 x 4096 15.0 / 14.8; 8 16.5 / 14.8; 8, 32000 x 2048 16.2 / 14.0).  Eight wavefronts share the k of a strip
+// where there are few strips (4096 x 14336 12.6, four of them 14.5), four where they fill the chip (128256 x 4096 85.3, eight 86.5).
+constexpr int OP_FEW_STRIPS = 512;
 template <typename TY>
 static void op_product_piece(hipStream_t s, const OpProductArgs<TY>& p) {
-    if (p.m <= 16) op_stream<TY, 1>(s, p);
-    else if (p.m <= 32) op_stream<TY, 2>(s, p);
-    else if (p.m <= 64) op_stream<TY, 4>(s, p);
-    else op_ring<TY>(s, p);
+    double ring_us;
+    const int tile = op_ring_pick(p.m, p.n, p.kp, sizeof(TY), &ring_us);
+    if (p.m > 32 || 4.0 + (double)p.n * p.kp / 6.6e6 * (1.0 + 0.042 * p.m) > ring_us) { op_ring<TY>(s, p, tile); return; }
+    const unsigned strips = (unsigned)op_cdiv(p.n, 16);
+#define OP_STREAM(MT, KS, D) hipLaunchKernelGGL((op_stream_kernel<TY, MT, KS, D>), dim3(strips), dim3(64 * KS), 0, s, p)
+    if (strips <= OP_FEW_STRIPS) { if (p.m <= 16) OP_STREAM(1, 8, 4); else OP_STREAM(2, 8, 4); }
+    else { if (p.m <= 16) OP_STREAM(1, 4, 8); else OP_STREAM(2, 4, 8); }
+#undef OP_STREAM
 }
 void op_product(hipStream_t s, const OpProduct& p, void*) {
     constexpr int64_t PM = 1 << 16, PN = 1 << 18;          // a launch's rows and channels: its tiles have 32-bit numbers
@@ -93,11 +97,26 @@ void op_product(hipStream_t s, const OpProduct& p, void*) {
     });
 }
 
+constexpr int OP_TOKEN_STRIPS = 2048;
 // workspace of a linear: codes of the rows, their scales, then what the product needs
 static uint64_t op_linear_codes(int64_t m, int32_t k) { return (uint64_t)m * op_code_ld(k); }
 static uint64_t op_linear_rows(int64_t m, int32_t k) { return op_linear_codes(m, k) + (uint64_t)op_cdiv(m, 4) * 16; }
-uint64_t op_linear_workspace(int64_t m, int64_t n, int32_t k) { return op_linear_rows(m, k) + op_product_workspace(m, n, k); }
+// one token whose row every workgroup quantises for itself: no workspace
+static bool op_token(int64_t m, int64_t n, int32_t k) { return m == 1 && n <= 16 * OP_TOKEN_STRIPS && k <= OP_ROW_E * 512; }
+uint64_t op_linear_workspace(int64_t m, int64_t n, int32_t k) { return op_token(m, n, k) ? 0 : op_linear_rows(m, k) + op_product_workspace(m, n, k); }
 void op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const OpProduct& p, void* workspace) {
+    if (op_token(p.m, p.n, p.k)) {
+        op_with_type(x_type, [&](auto tx) {
+            op_with_type(p.y_type, [&](auto ty) {
+                typedef decltype(tx) TX; typedef decltype(ty) TY;
+                const OpProductArgs<TY> a{nullptr, 0, nullptr, p.w, p.ldw, p.w_scale, p.bias, 1, (int)p.n, (int)op_code_ld(p.k), (TY*)p.y, p.ldy};
+                const dim3 grid((unsigned)op_cdiv(p.n, 16));
+                if (grid.x <= OP_FEW_STRIPS || p.k > OP_ROW_E * 256) hipLaunchKernelGGL((op_token_kernel<TX, TY, 8, 4>), grid, dim3(512), 0, s, a, (const TX*)x, p.k);
+                else hipLaunchKernelGGL((op_token_kernel<TX, TY, 4, 8>), grid, dim3(256), 0, s, a, (const TX*)x, p.k);
+            });
+        });
+        return;
+    }
     OpProduct q = p;
     int8_t* codes = (int8_t*)workspace;
     float* scale = (float*)(codes + op_linear_codes(p.m, p.k));

@@ -35,30 +35,99 @@ __device__ __forceinline__ int op_code(float v, float to_code) {
     return to_code == 0.f ? 0 : (int)__builtin_rintf(fminf(fmaxf(v * to_code, -127.f), 127.f));
 }
 
-template <typename T>
-static __global__ __launch_bounds__(256) void op_quantize_kernel(const T* __restrict__ x, int cols, int64_t ldx, int8_t* __restrict__ codes, int64_t ldq, float* __restrict__ scale) {
-    __shared__ uint32_t red[4];
-    const T* row = x + (int64_t)blockIdx.x * ldx;
-    int8_t* out = codes + (int64_t)blockIdx.x * ldq;
+// A thread's share of a row in registers: NV pieces of 16 bytes, NT pieces apart; zeros behind the row's end.
+template <typename T, int NV, int NT> struct OpRowPart {
+    static constexpr int V = 16 / (int)sizeof(T);
+    T x[NV][V];
+    __device__ __forceinline__ void load(const T* row, int k, int t) {
+        if (((uintptr_t)row & 15) == 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                const int c = (t + NT * i) * V;
+                if (c + V <= k) *reinterpret_cast<uint4*>(x[i]) = *reinterpret_cast<const uint4*>(row + c);
+                else
+#pragma unroll
+                    for (int e = 0; e < V; ++e) x[i][e] = c + e < k ? row[c + e] : op_cast<T>(0.f);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int e = 0; e < V; ++e) { const int c = (t + NT * i) * V + e; x[i][e] = c < k ? row[c] : op_cast<T>(0.f); }
+        }
+    }
+    __device__ __forceinline__ uint32_t largest() const {          // of the wavefront
+        uint32_t mag = 0;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int e = 0; e < V; ++e) mag = max(mag, op_mag(op_f32<T>(x[i][e])));
+        for (int d = 32; d; d >>= 1) mag = max(mag, (uint32_t)__shfl_xor((int)mag, d));
+        return mag;
+    }
+    __device__ __forceinline__ void store(int8_t* codes, int kp, int t, float to_code) const {          // kp: the row's end with its zeros
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int c = (t + NT * i) * V;
+            if (c >= kp) continue;
+            uint32_t w[V / 4];
+#pragma unroll
+            for (int e = 0; e < V; ++e) w[e / 4] = (e % 4 ? w[e / 4] : 0u) | (uint32_t)(uint8_t)op_code(op_f32<T>(x[i][e]), to_code) << 8 * (e % 4);
+#pragma unroll
+            for (int e = 0; e < V / 4; ++e) reinterpret_cast<uint32_t*>(codes + c)[e] = w[e];
+        }
+    }
+};
+// W wavefronts a row, 4 / W rows a workgroup (one where W > 4); the row stays in registers between its largest value and its codes: one read, one write.
+// kp <= OP_ROW_E x 64 W.  (Two passes over memory, one element a thread and step: 8192 columns of one row 11.5 us in front of a product, 2041 x 4096 bfloat16 12.8.)
+constexpr int OP_ROW_E = 32;
+template <typename T, int W>
+static __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void op_quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int8_t* __restrict__ codes, int64_t ldq, float* __restrict__ scale) {
+    __shared__ uint32_t red[W > 4 ? W : 4];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x & (64 * W - 1);
+    const int64_t row = (int64_t)blockIdx.x * (W > 4 ? 1 : 4 / W) + wave / W;
+    const bool live = row < rows;
+    OpRowPart<T, OP_ROW_E * (int)sizeof(T) / 16, 64 * W> part;
     uint32_t mag = 0;
-    for (int c = threadIdx.x; c < cols; c += 256) mag = max(mag, op_mag(op_f32<T>(row[c])));
-    for (int d = 32; d; d >>= 1) mag = max(mag, (uint32_t)__shfl_xor((int)mag, d));
+    if (live) {
+        part.load(x + row * ldx, cols, t);
+        mag = part.largest();
+    }
+    if constexpr (W > 1) {
+        if ((threadIdx.x & 63) == 0) red[wave] = mag;
+        __syncthreads();
+        mag = 0;
+#pragma unroll
+        for (int i = 0; i < W; ++i) mag = max(mag, red[wave / W * W + i]);
+    }
+    if (!live) return;
+    float s, r;
+    op_row_scale(mag, s, r);
+    if (t == 0) scale[row] = s;
+    part.store(codes + row * ldq, (cols + GL3_CODE_BLOCK - 1) / GL3_CODE_BLOCK * GL3_CODE_BLOCK, t, r);
+}
+// longer rows: read twice
+template <typename T>
+static __global__ __launch_bounds__(1024) void op_quantize_long_kernel(const T* __restrict__ x, int cols, int64_t ldx, int8_t* __restrict__ codes, int64_t ldq, float* __restrict__ scale) {
+    __shared__ uint32_t red[16];
+    constexpr int STEP = OP_ROW_E / 2 * 1024;
+    const T* row = x + (int64_t)blockIdx.x * ldx;
+    const int kp = (cols + GL3_CODE_BLOCK - 1) / GL3_CODE_BLOCK * GL3_CODE_BLOCK;
+    OpRowPart<T, OP_ROW_E / 2 * (int)sizeof(T) / 16, 1024> part;
+    uint32_t mag = 0;
+    for (int c = 0; c < cols; c += STEP) { part.load(row + c, cols - c, threadIdx.x); mag = max(mag, part.largest()); }
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mag;
     __syncthreads();
-    mag = max(max(red[0], red[1]), max(red[2], red[3]));
+#pragma unroll
+    for (int i = 0; i < 16; ++i) mag = max(mag, red[i]);
     float s, r;
     op_row_scale(mag, s, r);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
-    const int end = (cols + GL3_CODE_BLOCK - 1) / GL3_CODE_BLOCK * GL3_CODE_BLOCK;
-    for (int c = threadIdx.x; c < end; c += 256) out[c] = c < cols ? (int8_t)op_code(op_f32<T>(row[c]), r) : (int8_t)0;
+    for (int c = 0; c < kp; c += STEP) { part.load(row + c, cols - c, threadIdx.x); part.store(codes + (int64_t)blockIdx.x * ldq + c, kp - c, threadIdx.x, r); }
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float op_result(int acc, float as, float ws) { return ((float)acc * as) * ws; }
-template <bool ONCE> __device__ __forceinline__ op_v4i op_load16(const int8_t* p) {
-    const op_v4i* q = reinterpret_cast<const op_v4i*>(p);
-    return ONCE ? __builtin_nontemporal_load(q) : *q;
-}
 template <typename TY> struct OpProductArgs {
     const int8_t* a; int64_t lda; const float* as;
     const int8_t* w; int64_t ldw; const float* ws; const float* bias;
@@ -66,80 +135,121 @@ template <typename TY> struct OpProductArgs {
     TY* y; int64_t ldy;
 };
 
-// Up to 64 tokens: the weights' bytes are what it costs, and they go from memory to the matrix cores' registers directly.  A wavefront has 16 RT
-// channels x 16 MT tokens (v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l % 16) and a ring of D steps of 64 k on their way; the
-// tokens' codes come from the caches.  KS wavefronts of a workgroup share the channels and split k (their int32 sums meet in LDS: exact in any
-// order); KS = 1: four wavefronts with channels of their own.
-template <typename TY, int RT, int MT, int KS, int D, bool ONCE>
-static __global__ __launch_bounds__(64 * (KS == 1 ? 4 : KS)) void op_stream_kernel(OpProductArgs<TY> p) {
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), r16 = lane & 15, kg = lane >> 4;
-    const int n0 = (KS == 1 ? (int)blockIdx.x * 4 + wave : (int)blockIdx.x) * 16 * RT;
-    if (KS == 1 && n0 >= p.n) return;
-    const int steps = p.kp / 64, s0 = KS == 1 ? 0 : (int)((int64_t)steps * wave / KS), cnt = (KS == 1 ? steps : (int)((int64_t)steps * (wave + 1) / KS)) - s0;
-    const int8_t *wb = p.w + (int64_t)n0 * p.ldw + (int64_t)s0 * 64, *ab = p.a + (int64_t)s0 * 64;          // (uniform; the lanes' parts fit 32 bits)
-    uint32_t wo[RT], ao[MT];
+// A few tokens: the weights' bytes are what it costs, and they go from memory to the matrix cores' registers directly.  A wavefront has 16 channels
+// x 16 MT tokens (v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l % 16) and a ring of D steps of 64 k on their way; the KS wavefronts of a
+// workgroup share the channels and split k (their int32 sums meet in LDS: exact in any order).  The tokens' codes come from the caches, which costs
+// 4 % of the weights' time a token (128256 x 4096, us: 1 token 85, 4 95, 16 144, 32 197; tiles 88, 92, 98, 102): op_product_piece compares.
+// (Loads past the caches fetch the 128-byte lines twice, half by half: 85 -> 95.  32 or 64 channels a wavefront: 92, 97.)
+template <int KS> struct OpStrip {          // the wavefront's part of a strip of 16 channels
+    int lane, wave, r16, kg, n0, s0, cnt;
+    const int8_t* wb;
+    uint32_t wo;
+    __device__ __forceinline__ OpStrip(const int8_t* w, int64_t ldw, int n, int kp) {
+        lane = threadIdx.x & 63; wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); r16 = lane & 15; kg = lane >> 4;
+        const int steps = kp / 64;
+        s0 = steps * wave / KS; cnt = steps * (wave + 1) / KS - s0;
+        n0 = (int)blockIdx.x * 16;
+        wb = w + n0 * ldw + s0 * 64;          // (uniform; the lane's part fits 32 bits; rows past the end repeat the last one)
+        wo = (uint32_t)(min(n0 + r16, n - 1) - n0) * (uint32_t)ldw + 16 * kg;
+    }
+    __device__ __forceinline__ op_v4i load(int s) const { return *reinterpret_cast<const op_v4i*>(wb + s * 64 + wo); }
+};
+// lane: token r16 of tile j, channels 4 kg .. of the strip
+template <typename TY> __device__ __forceinline__ void op_store4(const OpProductArgs<TY>& p, const op_v4i& v, int row, int col, float sa) {
+    if (row >= p.m) return;
 #pragma unroll
-    for (int i = 0; i < RT; ++i) wo[i] = (uint32_t)(min(n0 + 16 * i + r16, p.n - 1) - n0) * (uint32_t)p.ldw + 16 * kg;          // (rows past the end repeat the last one)
+    for (int r = 0; r < 4; ++r)
+        if (col + r < p.n) {
+            const float x = op_result(v[r], sa, p.ws[col + r]);
+            p.y[(int64_t)row * p.ldy + col + r] = op_cast<TY>(p.bias ? x + p.bias[col + r] : x);
+        }
+}
+template <typename TY, int MT, int KS, int D>
+static __global__ __launch_bounds__(64 * KS) void op_stream_kernel(OpProductArgs<TY> p) {
+    __shared__ op_v4i part[KS][MT][64];
+    const OpStrip<KS> st(p.w, p.ldw, p.n, p.kp);
+    const int8_t* ab = p.a + st.s0 * 64;
+    uint32_t ao[MT];
 #pragma unroll
-    for (int j = 0; j < MT; ++j) ao[j] = (uint32_t)min(16 * j + r16, p.m - 1) * (uint32_t)p.lda + 16 * kg;
-    op_v4i acc[RT][MT], fw[D][RT], fa[D][MT];
+    for (int j = 0; j < MT; ++j) ao[j] = (uint32_t)min(16 * j + st.r16, p.m - 1) * (uint32_t)p.lda + 16 * st.kg;
+    op_v4i acc[MT], fw[D], fa[D][MT];
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int j = 0; j < MT; ++j) acc[i][j] = op_v4i{0, 0, 0, 0};
+    for (int j = 0; j < MT; ++j) acc[j] = op_v4i{0, 0, 0, 0};
     auto load = [&](int d, int s) {
-        const int8_t *w = wb + (int64_t)s * 64, *a = ab + (int64_t)s * 64;
+        fw[d] = st.load(s);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) fw[d][i] = op_load16<ONCE>(w + wo[i]);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) fa[d][j] = op_load16<false>(a + ao[j]);
+        for (int j = 0; j < MT; ++j) fa[d][j] = *reinterpret_cast<const op_v4i*>(ab + s * 64 + ao[j]);
     };
     auto mma = [&](int d) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < MT; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[d][i], fa[d][j], acc[i][j], 0, 0, 0);
+        for (int j = 0; j < MT; ++j) acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[d], fa[d][j], acc[j], 0, 0, 0);
     };
-    if (cnt > 0) {
+    if (st.cnt > 0) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) load(d, min(d, cnt - 1));
+        for (int d = 0; d < D; ++d) load(d, min(d, st.cnt - 1));
         int s = 0;
-        for (; s + D < cnt; s += D)
+        for (; s + D < st.cnt; s += D)
 #pragma unroll
-            for (int d = 0; d < D; ++d) { mma(d); load(d, min(s + D + d, cnt - 1)); }
+            for (int d = 0; d < D; ++d) { mma(d); load(d, min(s + D + d, st.cnt - 1)); }
 #pragma unroll
-        for (int d = 0; d < D; ++d) if (s + d < cnt) mma(d);
+        for (int d = 0; d < D; ++d) if (s + d < st.cnt) mma(d);
     }
-    auto store = [&](const op_v4i& v, int i, int j) {          // lane: token l % 16, channels 4 (l / 16) ..
-        const int row = 16 * j + r16, col = n0 + 16 * i + 4 * kg;
-        if (row >= p.m) return;
-        const float sa = p.as[row];
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (col + r < p.n) {
-                const float x = op_result(v[r], sa, p.ws[col + r]);
-                p.y[(int64_t)row * p.ldy + col + r] = op_cast<TY>(p.bias ? x + p.bias[col + r] : x);
+    for (int j = 0; j < MT; ++j) part[st.wave][j][st.lane] = acc[j];
+    __syncthreads();
+    if (st.wave >= MT) return;
+    op_v4i v = part[0][st.wave][st.lane];
+#pragma unroll
+    for (int q = 1; q < KS; ++q) v += part[q][st.wave][st.lane];
+    const int row = 16 * st.wave + st.r16;
+    op_store4(p, v, row, st.n0 + 4 * st.kg, p.as[min(row, p.m - 1)]);
+}
+
+// One token of a linear: every workgroup quantises the row for itself (LDS) while its first weights are on their way, and one launch is all.  That costs each
+// of them about a microsecond, more than the launch where they run in many rounds (us, this / a launch of its own for the codes: 2048 x 2048 5.0 / 8.0, 14336 x 4096
+// 15.0 / 18.0, 32000 x 2048 16.6 / 16.9, 128256 x 4096 95 / 89; several strips a workgroup 100).  k <= OP_ROW_E x threads: the row stays in registers.
+template <typename TX, typename TY, int KS, int D>
+static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<TY> p, const TX* __restrict__ x, int k) {
+    constexpr int NT = 64 * KS;
+    __shared__ __attribute__((aligned(16))) int8_t codes[OP_ROW_E * NT];
+    __shared__ op_v4i sums[KS][64];
+    __shared__ uint32_t red[KS];
+    const OpStrip<KS> st(p.w, p.ldw, p.n, p.kp);
+    // the row first: loads come back in order, and the weights behind it do not hold it up
+    OpRowPart<TX, OP_ROW_E * (int)sizeof(TX) / 16, NT> part;
+    part.load(x, k, threadIdx.x);
+    op_v4i acc = {0, 0, 0, 0}, fw[D];
+#pragma unroll
+    for (int d = 0; d < D; ++d) fw[d] = st.load(max(0, min(d, st.cnt - 1)));
+    uint32_t mag = part.largest();
+    if (st.lane == 0) red[st.wave] = mag;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < KS; ++q) mag = max(mag, red[q]);
+    float scale, to_code;
+    op_row_scale(mag, scale, to_code);
+    part.store(codes, p.kp, threadIdx.x, to_code);
+    __syncthreads();
+    const int8_t* cb = codes + st.s0 * 64 + 16 * st.kg;          // (all 16 token columns are this token)
+    if (st.cnt > 0) {
+        int s = 0;
+        for (; s + D < st.cnt; s += D)
+#pragma unroll
+            for (int d = 0; d < D; ++d) {
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[d], *reinterpret_cast<const op_v4i*>(cb + (s + d) * 64), acc, 0, 0, 0);
+                fw[d] = st.load(min(s + D + d, st.cnt - 1));
             }
-    };
-    if constexpr (KS == 1) {
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < MT; ++j) store(acc[i][j], i, j);
-    } else {
-        __shared__ op_v4i part[KS][RT * MT][64];
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-            for (int j = 0; j < MT; ++j) part[wave][i * MT + j][lane] = acc[i][j];
-        __syncthreads();
-        for (int t = wave; t < RT * MT; t += KS) {
-            op_v4i v = part[0][t][lane];
-#pragma unroll
-            for (int q = 1; q < KS; ++q) v += part[q][t][lane];
-            store(v, t / MT, t % MT);
-        }
+        for (int d = 0; d < D; ++d)
+            if (s + d < st.cnt) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[d], *reinterpret_cast<const op_v4i*>(cb + (s + d) * 64), acc, 0, 0, 0);
     }
+    sums[st.wave][st.lane] = acc;
+    __syncthreads();
+    if (st.wave) return;
+    op_v4i v = sums[0][st.lane];
+#pragma unroll
+    for (int q = 1; q < KS; ++q) v += sums[q][st.lane];
+    op_store4(p, v, st.r16, st.n0 + 4 * st.kg, scale);
 }
 
 // More tokens: BM tokens x BN channels per workgroup of WM x WN wavefronts, v_mfma_i32_32x32x32_i8.  The operands go straight to LDS (16 bytes a lane, no

@@ -19,15 +19,30 @@ from . import hip
 CODE_BLOCK = 128             # GL3_CODE_BLOCK
 MAX_K = 131071               # GL3_INT8_MAX_K
 MAX_TOP = 64                 # GL3_LOGPROBS_MAX_TOP
+
+
+def _bad(what):
+    return hip.Gl3Error(hip.E_ARG, what)
+
+
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
-class Int8Rows(NamedTuple):
+class Int8Rows:
     """Rows of int8 codes with a scale each; row i stands for codes[i, :cols] * scale[i].  codes: int8 [rows, ld], ld >= cols rounded up to a
-    multiple of CODE_BLOCK and a multiple of 16, zeros from column cols to that multiple; scale: float32 [rows]."""
-    codes: torch.Tensor
-    scale: torch.Tensor
-    cols: int
+    multiple of CODE_BLOCK, rows that start on 16 bytes, zeros from column cols to that multiple; scale: float32 [rows].  Checked once, here."""
+    __slots__ = ("codes", "scale", "cols", "rows", "ld", "device")
+
+    def __init__(self, codes: torch.Tensor, scale: torch.Tensor, cols: int):
+        if codes.dim() != 2 or codes.dtype != torch.int8 or (codes.stride(1) != 1 and codes.shape[1] != 1):
+            raise _bad("codes must be an int8 matrix with contiguous rows")
+        if not 0 < cols <= MAX_K or codes.shape[1] < -(-cols // CODE_BLOCK) * CODE_BLOCK:
+            raise _bad("a row of codes is %d columns and zeros up to a multiple of %d, at most %d" % (cols, CODE_BLOCK, MAX_K))
+        if scale.dim() != 1 or scale.shape[0] != codes.shape[0] or scale.dtype != torch.float32 or scale.device != codes.device or not scale.is_contiguous():
+            raise _bad("scale must hold one float32 per row of codes, beside them")
+        self.codes, self.scale, self.cols = codes, scale, cols
+        self.rows, self.device = codes.shape[0], codes.device
+        self.ld = codes.stride(0) if self.rows > 1 else codes.shape[1] // 16 * 16
 
     def dequantize(self, dtype=torch.float32) -> torch.Tensor:
         return (self.codes[:, :self.cols].float() * self.scale[:, None]).to(dtype)
@@ -43,31 +58,23 @@ class TokenLogprobs(NamedTuple):
     top_logprobs: Optional[torch.Tensor]
 
 
-def _need(ok, what):
-    if not ok:
-        raise hip.Gl3Error(hip.E_ARG, what)
-
-
 def _rows(x, name):
     """A float matrix on a GPU whose rows are contiguous -> its row stride."""
-    _need(x.is_cuda, name + " must be on a GPU: there is no CPU path")
-    _need(x.dim() == 2 and x.dtype in _TYPES, name + " must be a matrix of float32, float16 or bfloat16")
-    _need(x.stride(1) == 1 or x.shape[1] == 1, name + ": the elements of a row must be contiguous")
-    _need(not (x.requires_grad and torch.is_grad_enabled()), name + " requires a gradient: these operators are forward only")
-    return x.stride(0)
+    if not x.is_cuda:
+        raise _bad(name + " must be on a GPU: there is no CPU path")
+    if x.dim() != 2 or x.dtype not in _TYPES:
+        raise _bad(name + " must be a matrix of float32, float16 or bfloat16")
+    rows, inner = x.stride()
+    if inner != 1 and x.shape[1] != 1:
+        raise _bad(name + ": the elements of a row must be contiguous")
+    if x.requires_grad and torch.is_grad_enabled():
+        raise _bad(name + " requires a gradient: these operators are forward only")
+    return rows
 
 
 def _like(t, name, shape, dtype, device):
-    _need(t.shape == shape and t.dtype == dtype and t.device == device and t.is_contiguous(), "%s must be a contiguous %s tensor of shape %s on %s" % (name, dtype, tuple(shape), device))
-
-
-def _codes(r, name, device):
-    c = r.codes
-    _need(c.dim() == 2 and c.dtype == torch.int8 and c.device == device and c.stride(1) == 1, name + ".codes must be an int8 matrix with contiguous rows on " + str(device))
-    _need(0 < r.cols <= MAX_K and c.shape[1] >= -(-r.cols // CODE_BLOCK) * CODE_BLOCK, name + ".codes: a row is cols columns and zeros up to a multiple of %d" % CODE_BLOCK)
-    s = r.scale
-    _need(s.dim() == 1 and s.shape[0] == c.shape[0] and s.dtype == torch.float32 and s.device == device and s.is_contiguous(), name + ".scale must hold one float32 per row on " + str(device))
-    return c.stride(0) if c.shape[0] > 1 else c.shape[1]
+    if t.shape != shape or t.dtype != dtype or t.device != device or not t.is_contiguous():
+        raise _bad("%s must be a contiguous %s tensor of shape %s on %s" % (name, dtype, tuple(shape), device))
 
 
 @functools.lru_cache(maxsize=4096)
@@ -103,38 +110,41 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     scale 0; a row with a NaN or an infinity has scale NaN."""
     ld = _rows(x, "x")
     rows, cols = x.shape
-    _need(0 < cols <= MAX_K, "x must have 1 .. %d columns" % MAX_K)
-    codes = torch.empty(rows, -(-cols // CODE_BLOCK) * CODE_BLOCK, dtype=torch.int8, device=x.device)
-    scale = torch.empty(rows, dtype=torch.float32, device=x.device)
-    _call(hip.lib().gl3_quantize_rows, x.device, x.data_ptr(), _TYPES[x.dtype], rows, cols, ld, codes.data_ptr(), codes.shape[1], scale.data_ptr())
+    if not 0 < cols <= MAX_K:
+        raise _bad("x must have 1 .. %d columns" % MAX_K)
+    device = x.device
+    codes = torch.empty(rows, -(-cols // CODE_BLOCK) * CODE_BLOCK, dtype=torch.int8, device=device)
+    scale = torch.empty(rows, dtype=torch.float32, device=device)
+    _call(hip.lib().gl3_quantize_rows, device, x.data_ptr(), _TYPES[x.dtype], rows, cols, ld, codes.data_ptr(), codes.shape[1], scale.data_ptr())
     return Int8Rows(codes, scale, cols)
 
 
-def _product(w, bias, m, k, dtype, out, device):
-    ldw = _codes(w, "w", device)
-    n = w.codes.shape[0]
-    _need(w.cols == k, "the rows have %d columns, the weights %d" % (k, w.cols))
-    _need(dtype in _TYPES, "results are float32, float16 or bfloat16")
+def _result(w, bias, m, k, dtype, out, device):
+    n = w.rows
+    if w.cols != k or w.device != device:
+        raise _bad("the rows have %d columns on %s, the weights %d on %s" % (k, device, w.cols, w.device))
+    if dtype not in _TYPES:
+        raise _bad("results are float32, float16 or bfloat16")
     if bias is not None:
         _like(bias, "bias", (n,), torch.float32, device)
     if out is None:
-        out = torch.empty(m, n, dtype=dtype, device=device)
-    else:
-        _need(out.shape == (m, n) and out.dtype == dtype and out.device == device and (out.stride(1) == 1 or n == 1), "out must be a %d x %d matrix of %s with contiguous rows on %s" % (m, n, dtype, device))
-    return ldw, n, out
+        return torch.empty(m, n, dtype=dtype, device=device), n
+    if out.shape != (m, n) or out.dtype != dtype or out.device != device or (out.stride(1) != 1 and n != 1):
+        raise _bad("out must be a %d x %d matrix of %s with contiguous rows on %s" % (m, n, dtype, device))
+    return out, out.stride(0)
 
 
 def int8_matmul(a: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None, dtype=torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[i, j] = (sum_k a[i, k] w[j, k]) * a.scale[i] * w.scale[j] (+ bias[j]): the sum exact in int32, one rounding to dtype."""
-    device = a.codes.device
-    _need(device.type == "cuda", "a must be on a GPU: there is no CPU path")
-    lda = _codes(a, "a", device)
-    m, k = a.codes.shape[0], a.cols
-    ldw, n, out = _product(w, bias, m, k, dtype, out, device)
+    device = a.device
+    if device.type != "cuda":
+        raise _bad("a must be on a GPU: there is no CPU path")
+    m, k, n = a.rows, a.cols, w.rows
+    out, ldy = _result(w, bias, m, k, dtype, out, device)
     nbytes = _int8_bytes(m, n, k)[0]
     ws = _workspace(nbytes, device)
-    _call(hip.lib().gl3_int8_matmul, device, a.codes.data_ptr(), lda, a.scale.data_ptr(), w.codes.data_ptr(), ldw, w.scale.data_ptr(), _ptr(bias), m, n, k,
-          out.data_ptr(), _TYPES[dtype], out.stride(0), _ptr(ws), nbytes)
+    _call(hip.lib().gl3_int8_matmul, device, a.codes.data_ptr(), a.ld, a.scale.data_ptr(), w.codes.data_ptr(), w.ld, w.scale.data_ptr(), _ptr(bias), m, n, k,
+          out.data_ptr(), _TYPES[dtype], ldy, _ptr(ws), nbytes)
     return out
 
 
@@ -142,13 +152,15 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, bias: Optional[torch.Tensor] = Non
     """int8_matmul(quantize_rows(x), w, bias), bit for bit, in as few launches as the sizes allow.  dtype: of the result (default: x's)."""
     ldx = _rows(x, "x")
     m, k = x.shape
+    n = w.rows
     device = x.device
-    dtype = x.dtype if dtype is None else dtype
-    ldw, n, out = _product(w, bias, m, k, dtype, out, device)
+    if dtype is None:
+        dtype = x.dtype
+    out, ldy = _result(w, bias, m, k, dtype, out, device)
     nbytes = _int8_bytes(m, n, k)[1]
     ws = _workspace(nbytes, device)
-    _call(hip.lib().gl3_int8_linear, device, x.data_ptr(), _TYPES[x.dtype], ldx, w.codes.data_ptr(), ldw, w.scale.data_ptr(), _ptr(bias), m, n, k,
-          out.data_ptr(), _TYPES[dtype], out.stride(0), _ptr(ws), nbytes)
+    _call(hip.lib().gl3_int8_linear, device, x.data_ptr(), _TYPES[x.dtype], ldx, w.codes.data_ptr(), w.ld, w.scale.data_ptr(), _ptr(bias), m, n, k,
+          out.data_ptr(), _TYPES[dtype], ldy, _ptr(ws), nbytes)
     return out
 
 
@@ -158,7 +170,8 @@ def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None,
     ld = _rows(logits, "logits")
     rows, vocab = logits.shape
     device = logits.device
-    _need(vocab > 0 and 0 <= top <= MAX_TOP, "vocab must be positive, top in 0 .. %d" % MAX_TOP)
+    if vocab < 1 or not 0 <= top <= MAX_TOP:
+        raise _bad("vocab must be positive, top in 0 .. %d" % MAX_TOP)
     logprob = rank = ent = ids = values = None
     if targets is not None:
         _like(targets, "targets", (rows,), torch.int32, device)
