@@ -628,6 +628,7 @@ int32_t gl3_create(const gl3_model_desc* desc, gl3_ctx** out) {
         if ((d.flags & GL3_FLAG_VECTOR_512) && d.weight_type == GL3_TYPE_F16 && d.tp_size > 1)
             return bail(GL3_E_UNSUPPORTED, "the 512-bit F16 species is built for one rank");
     }
+    if (d.flags & GL3_FLAG_INT8_HEAD) return bail(GL3_E_UNSUPPORTED, "GL3_FLAG_INT8_HEAD: the GGUF families' logits are the reference's bit for bit");
     if ((d.flags & GL3_FLAG_F32_ACTIVATION) && d.weight_type != GL3_TYPE_Q8_0)
         return bail(GL3_E_ARG, "GL3_FLAG_F32_ACTIVATION applies to Q8_0 matrices");
     if (q8v && (d.flags & GL3_FLAG_SCALAR_DOT))
@@ -1495,10 +1496,28 @@ int32_t gl3_reset_kv(gl3_ctx* ctx) {
 
 // The general step (include/gpullama3_hip.h).  Families without a kernel path that returns logits from inside a portion run the wanted
 // rows as decode steps and the runs between them as batched prefill.
-int32_t gl3_forward_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want, float* logits_out) {
-    if (!ctx) return GL3_E_ARG;
-    if (ctx->hy) return gl3_hy_step(ctx, seq, tokens, n, start_pos, want, n_want, logits_out);
-    if (!tokens || n < 1 || n_want < 0 || (n_want > 0 && (!want || !logits_out))) GL3_FAIL(GL3_E_ARG, "bad step arguments");
+}  // extern "C"
+
+// One decode step whose logits stay on the device; their scores for wanted row `row` of a call.
+static int32_t score_decode(gl3_ctx* ctx, int32_t token, int32_t pos, const gl3_score& score, int row) {
+    int32_t r = set_dyn(ctx, token, pos);
+    if (r != GL3_OK) return r;
+    if ((r = gl3_score_alloc(ctx, 1)) != GL3_OK) return r;
+    gl3_drain drain{ctx->stream};
+    const int amode = attn_mode(ctx, pos);
+    if (ctx->graph_exec) GL3_HIP(hipGraphLaunch(step_graph(ctx, amode), ctx->stream));
+    else if ((r = enqueue_decode(ctx, true, nullptr, amode)) != GL3_OK) return r;
+    if ((r = gl3_score_enqueue(ctx, score, row, 1, ctx->logits)) != GL3_OK) return r;
+    GL3_HIP(hipStreamSynchronize(ctx->stream));
+    drain.passed = true;
+    if ((r = gl3_tp_check(ctx)) != GL3_OK) return r;
+    gl3_score_collect(ctx, score, row, 1);
+    return GL3_OK;
+}
+
+// The general step of the GGUF families, composed of their calls: runs of tokens as batched prefill, wanted rows as decode steps.
+template <typename F>
+static int32_t composed_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want, F&& wanted_row) {
     if (seq != 0) GL3_FAIL(GL3_E_UNSUPPORTED, "gl3_forward_step: this family steps sequence 0 only");
     int run0 = 0, wi = 0;
     const int mb = ctx->d.max_batch > 1 ? ctx->d.max_batch : 1;
@@ -1512,13 +1531,36 @@ int32_t gl3_forward_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32
             run0 = i + 1;
         }
         if (wanted) {
-            const int32_t r = gl3_forward_decode(ctx, tokens[i], start_pos + i, logits_out + (size_t)wi * ctx->d.vocab, nullptr);
+            const int32_t r = wanted_row(i, wi);
             if (r != GL3_OK) return r;
             ++wi;
         }
     }
     if (wi != n_want) GL3_FAIL(GL3_E_ARG, "want must be ascending indices into the step's tokens");
     return GL3_OK;
+}
+
+extern "C" {
+
+int32_t gl3_forward_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want, float* logits_out) {
+    if (!ctx) return GL3_E_ARG;
+    if (ctx->hy) return gl3_hy_step(ctx, seq, tokens, n, start_pos, want, n_want, logits_out);
+    if (!tokens || n < 1 || n_want < 0 || (n_want > 0 && (!want || !logits_out))) GL3_FAIL(GL3_E_ARG, "bad step arguments");
+    return composed_step(ctx, seq, tokens, n, start_pos, want, n_want,
+                         [&](int i, int wi) { return gl3_forward_decode(ctx, tokens[i], start_pos + i, logits_out + (size_t)wi * ctx->d.vocab, nullptr); });
+}
+
+int32_t gl3_forward_score(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want, const int32_t* targets, int32_t top,
+                          float* logprobs, int32_t* ranks, float* entropies, int32_t* top_ids, float* top_logprobs) {
+    if (!ctx) return GL3_E_ARG;
+    const gl3_score score{targets, top, logprobs, ranks, entropies, top_ids, top_logprobs};
+    if (ctx->hy) return gl3_hy_step(ctx, seq, tokens, n, start_pos, want, n_want, nullptr, &score);
+    if (!tokens || n < 1 || n_want < 0 || (n_want > 0 && !want)) GL3_FAIL(GL3_E_ARG, "bad step arguments");
+    for (int32_t i = 0; i < n_want; ++i)
+        if (want[i] < 0 || want[i] >= n || (i && want[i] <= want[i - 1])) GL3_FAIL(GL3_E_ARG, "want must be ascending indices into the step's tokens");
+    const int32_t r = gl3_score_check(ctx, score, n_want);
+    if (r != GL3_OK) return r;
+    return composed_step(ctx, seq, tokens, n, start_pos, want, n_want, [&](int i, int wi) { return score_decode(ctx, tokens[i], start_pos + i, score, wi); });
 }
 
 int32_t gl3_seq_acquire(gl3_ctx* ctx, int32_t* seq_out) {

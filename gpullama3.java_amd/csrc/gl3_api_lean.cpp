@@ -65,6 +65,12 @@ int32_t gl3_forward_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32
     LEAN_CTX(ctx);
     return gl3_hy_step(ctx, seq, tokens, n, start_pos, want, n_want, logits_out);
 }
+int32_t gl3_forward_score(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want, const int32_t* targets, int32_t top,
+                          float* logprobs, int32_t* ranks, float* entropies, int32_t* top_ids, float* top_logprobs) {
+    LEAN_CTX(ctx);
+    const gl3_score score{targets, top, logprobs, ranks, entropies, top_ids, top_logprobs};
+    return gl3_hy_step(ctx, seq, tokens, n, start_pos, want, n_want, nullptr, &score);
+}
 int32_t gl3_seq_acquire(gl3_ctx* ctx, int32_t* seq_out) { LEAN_CTX(ctx); return seq_out ? gl3_hy_seq_acquire(ctx, seq_out) : GL3_E_ARG; }
 int32_t gl3_seq_release(gl3_ctx* ctx, int32_t seq) { LEAN_CTX(ctx); return gl3_hy_seq_release(ctx, seq); }
 int32_t gl3_get_layer_rows(gl3_ctx* ctx, int32_t layer, float* out, int32_t n) { LEAN_CTX(ctx); return gl3_hy_layer_rows(ctx, layer, out, n); }

@@ -182,6 +182,8 @@ struct gl3_ctx {
     int64_t topp_device = 0, topp_host = 0;       // top-p draws answered on the device / by the host heap (gl3_get_topp_counts)
     void* sm_sort = nullptr;                      // top-p on the device: (key, index) x 2, radix histogram, result words
     std::vector<int> topp_indices;
+    void *sc_dev = nullptr, *h_sc = nullptr;      // scores (gl3_sample.hip): targets, results and scratch of sc_rows rows; page-locked targets and results
+    int sc_rows = 0;
     std::vector<std::pair<void*, size_t>> pinned;     // caller buffers registered with gl3_pin_host_buffer (logits land there directly)
     // upload staging
     uint8_t* staging = nullptr;
@@ -258,6 +260,12 @@ int32_t gl3_tp_check(gl3_ctx* ctx);      // after a stream sync: GL3_E_RCCL if a
 // gl3_sample.hip
 int32_t gl3_sample_run(gl3_ctx* ctx, const float* logits_dev, float temperature, float topp, float coin, int32_t* token_out);
 int32_t gl3_sample_probs(gl3_ctx* ctx, float* out);
+// what gl3_forward_score asks of the wanted rows (host pointers of the whole call)
+struct gl3_score { const int32_t* targets; int32_t top; float* logprobs; int32_t* ranks; float* entropies; int32_t* top_ids; float* top_logprobs; };
+int32_t gl3_score_check(gl3_ctx* ctx, const gl3_score& s, int32_t n_want);
+int32_t gl3_score_alloc(gl3_ctx* ctx, int rows);                      // for at most `rows` rows at a time
+int32_t gl3_score_enqueue(gl3_ctx* ctx, const gl3_score& s, int first, int rows, const float* logits_dev);          // of wanted rows first ..; results on their way to page-locked memory
+void gl3_score_collect(gl3_ctx* ctx, const gl3_score& s, int first, int rows);                                    // behind a wait for the stream
 void gl3_sample_free(gl3_ctx* ctx);
 
 // gl3_prefill.hip

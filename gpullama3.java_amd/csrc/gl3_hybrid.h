@@ -114,6 +114,11 @@ struct gl3_hybrid_state {
     int *sel = nullptr, *pair_row = nullptr, *tiles = nullptr, *ntiles = nullptr;
     std::vector<HyLayer> L;
     HyMat emb, head;
+    // GL3_FLAG_INT8_HEAD: the head as codes [vocab][head_ldq] and a scale per row (head.w is gone then), scratch of its products
+    int8_t* head_q = nullptr;
+    float* head_s = nullptr;
+    int64_t head_ldq = 0;
+    void* head_ws = nullptr;
     float* final_norm = nullptr;
     HyHave have;
     // sequence slots: cache rows and recurrent state of every layer, [n_seqs][slot_floats]
@@ -153,7 +158,7 @@ void gl3_hy_destroy(gl3_ctx* ctx);                 // frees ctx->hy only
 int32_t gl3_hy_upload(gl3_ctx* ctx, int32_t id, int32_t layer, const void* host, uint64_t bytes, int32_t type);
 int32_t gl3_hy_finalize(gl3_ctx* ctx);
 int32_t gl3_hy_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want,
-                    float* logits_out);
+                    float* logits_out, const gl3_score* score = nullptr);          // score: what is read from the wanted rows instead (logits_out null)
 int32_t gl3_hy_argmax(gl3_ctx* ctx, int32_t* out);                  // greedy id of the last step's first wanted row
 int32_t gl3_hy_seq_acquire(gl3_ctx* ctx, int32_t* seq_out);
 int32_t gl3_hy_seq_release(gl3_ctx* ctx, int32_t seq);

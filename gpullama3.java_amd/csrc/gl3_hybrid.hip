@@ -28,6 +28,7 @@
 #include "gl3_hy_plain_kernels.h"
 #include "gl3_hy_pre_kernels.h"
 #include "gl3_hy_beside_kernels.h"
+#include "gl3_ops.h"
 
 using gl3::AMX_WGS;
 using gl3::argmax_kernel;
@@ -584,7 +585,7 @@ void gl3_hy_destroy(gl3_ctx* ctx) {
     if (!h) return;
     auto f = [](void* p) { if (p) hipFree(p); };
     auto hf = [](void* p) { if (p) hipHostFree(p); };
-    f(h->emb.w); f(h->head.w); f(h->final_norm);
+    f(h->emb.w); f(h->head.w); f(h->head_q); f(h->head_s); f(h->head_ws); f(h->final_norm);
     for (auto& L : h->L) {
         f(L.proj.w); f(L.o.w); f(L.gu.w); f(L.down.w); f(L.norm1); f(L.norm2); f(L.pbias);
         for (auto& q : L.hc) for (float* p : q) f(p);
@@ -926,6 +927,23 @@ int32_t gl3_hy_finalize(gl3_ctx* ctx) {
         HY_HIP(hipMemcpy(w.data(), h->final_norm, (size_t)h->W * 4, hipMemcpyDeviceToHost));
         for (float& v : w) v *= h->logit_mul;
         HY_HIP(hipMemcpy(h->final_norm, w.data(), (size_t)h->W * 4, hipMemcpyHostToDevice));
+    }
+    if (ctx->d.flags & GL3_FLAG_INT8_HEAD) {
+        const int V = h->head.rows, W = h->head.k;
+        const size_t es = h->f32 ? 4 : 2;
+        h->head_ldq = op_code_ld(W);
+        uint64_t ws = 0;
+        for (int m = 1; m <= h->want_cap; ++m) ws = std::max(ws, op_linear_workspace(m, V, W));
+        HY_HIP(hipMalloc((void**)&h->head_q, (size_t)V * h->head_ldq));
+        HY_HIP(hipMalloc((void**)&h->head_s, (size_t)V * 4));
+        HY_HIP(hipMalloc(&h->head_ws, std::max<uint64_t>(ws, 16)));
+        op_quantize(ctx->stream, h->head.w, h->f32 ? GL3_TYPE_F32 : GL3_TYPE_BF16, V, W, h->head.ld, h->head_q, h->head_ldq, h->head_s);
+        HY_HIP(hipGetLastError());
+        HY_HIP(hipStreamSynchronize(ctx->stream));
+        HY_HIP(hipFree(h->head.w));
+        h->head.w = nullptr;
+        h->mat_bytes -= (size_t)V * h->head.ld * es;
+        h->mat_bytes += (size_t)V * h->head_ldq;
     }
     HY_HIP(hipDeviceSynchronize());
     ctx->finalized = true;
@@ -1935,13 +1953,19 @@ static void hy_logits(gl3_ctx* ctx, int nw, bool normed = false) {          // o
     if (!normed) hy_streams<T>(ctx, nw, h->X, h->W, h->S, (size_t)h->mb * h->W, (const float*)nullptr, 1, 0, (const float*)nullptr, (const float*)nullptr,
                   h->ones, h->final_norm, ctx->d.rms_eps, xw, (float*)nullptr, h->want);
     HyGlu g{};
-    if (nw <= 4) g.cap = h->softcap;
-    if (nw == 1) {
+    if (h->head_q) {          // codes and a scale per vocabulary row; the normed rows are quantised in the same call
+        hy_pre_flush<T>(ctx);
+        h->leave = nullptr;
+        const OpProduct p{nullptr, 0, nullptr, h->head_q, h->head_ldq, h->head_s, nullptr, nw, h->head.rows, h->head.k, h->logits, GL3_TYPE_F32, ctx->d.vocab};
+        op_linear(ctx->stream, xw, sizeof(T) == 4 ? GL3_TYPE_F32 : GL3_TYPE_BF16, h->W, p, h->head_ws);
+    }
+    if (!h->head_q && nw <= 4) g.cap = h->softcap;
+    if (!h->head_q && nw == 1) {
         if (!hy_row_leaves<T>(h, xw, g)) h->leave = nullptr;
         g.host = h->leave;
     }
-    hy_gemm<T>(ctx, xw, h->W, h->head, nw, h->logits, ctx->d.vocab, false, nullptr, 0, g);
-    if (h->softcap > 0.f && nw > 4) {
+    if (!h->head_q) hy_gemm<T>(ctx, xw, h->W, h->head, nw, h->logits, ctx->d.vocab, false, nullptr, 0, g);
+    if (h->softcap > 0.f && (nw > 4 || h->head_q)) {
         const size_t cnt = (size_t)nw * ctx->d.vocab;
         hipLaunchKernelGGL(hy_softcap_kernel, dim3((unsigned)std::min<size_t>(1024, (cnt + 255) / 256)), dim3(256), 0, ctx->stream, h->logits, cnt, h->softcap);
     }
@@ -2151,7 +2175,7 @@ static int32_t hy_portion(gl3_ctx* ctx, int seq, const int32_t* tokens, int n, i
     return GL3_OK;
 }
 
-int32_t gl3_hy_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want, float* logits_out) {
+int32_t gl3_hy_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want, float* logits_out, const gl3_score* score) {
     gl3_hybrid_state* h = ctx->hy;
     if (!ctx->finalized) GL3_FAIL(GL3_E_STATE, "gl3_finalize has not run");
     if (seq < 0 || seq >= h->n_seqs) GL3_FAIL(GL3_E_ARG, "sequence slot out of range");
@@ -2163,7 +2187,9 @@ int32_t gl3_hy_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n,
         if (tokens[i] < 0 || tokens[i] >= ctx->d.vocab) GL3_FAIL(GL3_E_ARG, "token id out of range");
     for (int i = 0; i < n_want; ++i)
         if (want[i] < 0 || want[i] >= n || (i && want[i] <= want[i - 1])) GL3_FAIL(GL3_E_ARG, "want must be ascending indices into the step's tokens");
+    if (score) { const int32_t r = gl3_score_check(ctx, *score, n_want); if (r != GL3_OK) return r; }
     HY_HIP(hipSetDevice(ctx->d.device));
+    if (score && n_want > 0) { const int32_t r = gl3_score_alloc(ctx, h->want_cap); if (r != GL3_OK) return r; }
     gl3_drain drain{ctx->stream};
     const size_t V = ctx->d.vocab;
     int wi = 0;
@@ -2198,6 +2224,7 @@ int32_t gl3_hy_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n,
             }
             if (r != GL3_OK) return r;
             h->last_tok[seq] = tokens[off + pn - 1];
+            if (g > 0 && score && (r = gl3_score_enqueue(ctx, *score, done, g, h->logits)) != GL3_OK) return r;
             if (g > 0 && logits_out && !h->leave) {
                 launch_to_host(ctx, h->logits, h->h_logits, (size_t)g * V);
                 HY_HIP(hipGetLastError());
@@ -2208,6 +2235,7 @@ int32_t gl3_hy_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n,
                 h->rec ^= 1;
             } else HY_HIP(hipStreamSynchronize(ctx->stream));
             if (g > 0 && logits_out) memcpy(logits_out + (size_t)done * V, h->h_logits, (size_t)g * V * 4);
+            if (g > 0 && score) gl3_score_collect(ctx, *score, done, g);
             done += g;
         } while (done < we);
         wi = we;

@@ -29,6 +29,7 @@
 
 #include "gl3_ctx.h"
 #include "gl3_decode_kernels.h"
+#include "gl3_ops.h"
 
 using namespace gl3;
 
@@ -355,6 +356,9 @@ void gl3_sample_free(gl3_ctx* ctx) {
     if (ctx->sm_aux) hipFree(ctx->sm_aux);
     if (ctx->h_probs) hipHostFree(ctx->h_probs);
     if (ctx->sm_sort) hipFree(ctx->sm_sort);
+    if (ctx->sc_dev) hipFree(ctx->sc_dev);
+    if (ctx->h_sc) hipHostFree(ctx->h_sc);
+    ctx->sc_dev = nullptr; ctx->h_sc = nullptr; ctx->sc_rows = 0;
     ctx->sm_probs = nullptr; ctx->sm_aux = nullptr; ctx->h_probs = nullptr; ctx->sm_sort = nullptr;
 }
 
@@ -421,4 +425,60 @@ int32_t gl3_sample_probs(gl3_ctx* ctx, float* out) {       // parity tap: the pr
     if (!ctx->sm_probs) GL3_FAIL(GL3_E_STATE, "no sampled step yet");
     GL3_HIP(hipMemcpy(out, ctx->sm_probs, (size_t)ctx->d.vocab * 4, hipMemcpyDeviceToHost));
     return GL3_OK;
+}
+
+// ------------------------------------------------------------------------------------------------ scores (gl3_forward_score)
+// sc_dev: targets [rows], then the results of a group of rows (log probabilities, ranks, entropies, ids, their log probabilities, one behind the other), then
+// the operator's scratch; h_sc: page-locked targets and results.
+int32_t gl3_score_check(gl3_ctx* ctx, const gl3_score& s, int32_t n_want) {
+    if (s.top < 0 || s.top > GL3_LOGPROBS_MAX_TOP) GL3_FAIL(GL3_E_ARG, "top out of range (0 .. GL3_LOGPROBS_MAX_TOP)");
+    if ((s.targets != nullptr) != (s.logprobs != nullptr) || (s.targets != nullptr) != (s.ranks != nullptr)) GL3_FAIL(GL3_E_ARG, "targets, logprobs and ranks: all or none");
+    if (n_want > 0 && s.top > 0 && (!s.top_ids || !s.top_logprobs)) GL3_FAIL(GL3_E_ARG, "top > 0 needs top_ids and top_logprobs");
+    if (s.targets)
+        for (int32_t i = 0; i < n_want; ++i)
+            if (s.targets[i] >= ctx->d.vocab) GL3_FAIL(GL3_E_ARG, "target id out of range");
+    return GL3_OK;
+}
+static size_t score_words(int rows, int top) { return (size_t)rows * (3 + 2 * top); }
+int32_t gl3_score_alloc(gl3_ctx* ctx, int rows) {
+    if (ctx->sc_dev && ctx->h_sc && ctx->sc_rows >= rows) return GL3_OK;
+    if (ctx->sc_dev) hipFree(ctx->sc_dev);
+    if (ctx->h_sc) hipHostFree(ctx->h_sc);
+    ctx->sc_dev = nullptr; ctx->h_sc = nullptr; ctx->sc_rows = 0;
+    uint64_t scratch = 0;
+    for (int r = 1; r <= rows; ++r) scratch = std::max(scratch, op_logprobs_workspace(r, ctx->d.vocab, GL3_LOGPROBS_MAX_TOP));
+    const size_t words = (size_t)rows + score_words(rows, GL3_LOGPROBS_MAX_TOP);
+    GL3_HIP(hipMalloc(&ctx->sc_dev, (words + 3) / 4 * 16 + scratch));
+    GL3_HIP(hipHostMalloc(&ctx->h_sc, words * 4));
+    ctx->sc_rows = rows;
+    return GL3_OK;
+}
+int32_t gl3_score_enqueue(gl3_ctx* ctx, const gl3_score& s, int first, int rows, const float* logits_dev) {
+    const int R = ctx->sc_rows;
+    int32_t* h = (int32_t*)ctx->h_sc;
+    int32_t* targets = (int32_t*)ctx->sc_dev;
+    float* res = (float*)(targets + R);
+    void* scratch = (uint8_t*)ctx->sc_dev + ((size_t)R + score_words(R, GL3_LOGPROBS_MAX_TOP) + 3) / 4 * 16;
+    if (s.targets) {
+        memcpy(h, s.targets + first, (size_t)rows * 4);
+        GL3_HIP(hipMemcpyAsync(targets, h, (size_t)rows * 4, hipMemcpyHostToDevice, ctx->stream));
+    }
+    const OpLogprobs p{logits_dev, GL3_TYPE_F32, rows, ctx->d.vocab, ctx->d.vocab, s.targets ? targets : nullptr, s.top, res, (int32_t*)res + rows, res + 2 * (size_t)rows,
+                       (int32_t*)res + 3 * (size_t)rows, res + 3 * (size_t)rows + (size_t)rows * s.top};
+    op_logprobs(ctx->stream, p, scratch);
+    GL3_HIP(hipGetLastError());
+    GL3_HIP(hipMemcpyAsync(h + R, res, score_words(rows, s.top) * 4, hipMemcpyDeviceToHost, ctx->stream));
+    return GL3_OK;
+}
+void gl3_score_collect(gl3_ctx* ctx, const gl3_score& s, int first, int rows) {
+    const float* res = (const float*)ctx->h_sc + ctx->sc_rows;
+    if (s.targets) {
+        memcpy(s.logprobs + first, res, (size_t)rows * 4);
+        memcpy(s.ranks + first, res + rows, (size_t)rows * 4);
+    }
+    if (s.entropies) memcpy(s.entropies + first, res + 2 * (size_t)rows, (size_t)rows * 4);
+    if (s.top) {
+        memcpy(s.top_ids + (size_t)first * s.top, res + 3 * (size_t)rows, (size_t)rows * s.top * 4);
+        memcpy(s.top_logprobs + (size_t)first * s.top, res + 3 * (size_t)rows + (size_t)rows * s.top, (size_t)rows * s.top * 4);
+    }
 }

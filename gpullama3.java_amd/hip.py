@@ -19,6 +19,7 @@ ERR_NAMES = {0: "GL3_OK", -1: "GL3_E_ARG", -2: "GL3_E_UNSUPPORTED", -3: "GL3_E_O
 FLAG_NO_GRAPH, FLAG_LAYER_TAPS, FLAG_FORCE_RCCL, FLAG_SCALAR_DOT, FLAG_F32_ACTIVATION = 1, 2, 4, 8, 16
 FLAG_VECTOR_512, FLAG_VECTOR_128 = 32, 64      # -Dllama.VectorBitSize (default 256): see include/gpullama3_hip.h
 FLAG_F32_COMPUTE = 128                         # layer-list family: float32 matrices and products
+FLAG_INT8_HEAD = 256                           # layer-list family: the output head in 8-bit integers
 ARCH_NODITAR = ARCH_LAYERLIST = 6      # the layer-list family; its designs differ in parameters only
 TYPE_F32, TYPE_BF16 = 0, 30
 MIX_ATTENTION, MIX_LATENT, MIX_SSM, MIX_MEMORY = 0, 1, 2, 3
@@ -147,6 +148,8 @@ _SIGS = {  # symbol -> (restype, argtypes): exactly the declarations of include/
     "gl3_kquant_to_q8_0": (C.c_int32, [C.c_int32, C.c_void_p, C.c_uint64, C.c_void_p]),
     "gl3_load_gguf": (C.c_int32, [C.c_char_p, C.POINTER(ModelDesc), C.POINTER(C.c_void_p)]),
     "gl3_forward_step": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p]),
+    "gl3_forward_score": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_int32, C.c_void_p, C.c_void_p, C.c_void_p,
+                                      C.c_void_p, C.c_void_p]),
     "gl3_seq_acquire": (C.c_int32, [C.c_void_p, C.POINTER(C.c_int32)]),
     "gl3_seq_release": (C.c_int32, [C.c_void_p, C.c_int32]),
     "gl3_get_layer_rows": (C.c_int32, [C.c_void_p, C.c_int32, C.c_void_p, C.c_int32]),
@@ -216,3 +219,17 @@ def check(code, ctx=None):
     if code != GL3_OK:
         msg = lib().gl3_last_error(ctx)
         raise Gl3Error(code, msg.decode() if msg else "")
+
+
+def score_step(ctx, seq, tokens, start_pos, want, targets, top):
+    """gl3_forward_score over numpy arrays -> dict(logprobs, ranks: None without targets; entropies; top_ids, top_logprobs: None for top = 0), one row per wanted row."""
+    import numpy as np
+    p = lambda a: a.ctypes.data_as(C.c_void_p) if a is not None and a.size else None
+    t, w = np.ascontiguousarray(tokens, np.int32), np.ascontiguousarray(want, np.int32)
+    g = None if targets is None else np.ascontiguousarray(targets, np.int32)
+    if g is not None and g.shape != w.shape:
+        raise Gl3Error(E_ARG, "one target per wanted row")
+    r = {"logprobs": None if g is None else np.empty(w.size, np.float32), "ranks": None if g is None else np.empty(w.size, np.int32), "entropies": np.empty(w.size, np.float32),
+         "top_ids": np.empty((w.size, top), np.int32) if top > 0 else None, "top_logprobs": np.empty((w.size, top), np.float32) if top > 0 else None}
+    check(lib().gl3_forward_score(ctx, seq, p(t), t.size, start_pos, p(w), w.size, p(g), top, p(r["logprobs"]), p(r["ranks"]), p(r["entropies"]), p(r["top_ids"]), p(r["top_logprobs"])), ctx)
+    return r

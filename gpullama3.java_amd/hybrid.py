@@ -66,7 +66,7 @@ class HybridPlan:
 
     @classmethod
     def from_dir(cls, path: str, dtype: str = "bfloat16", ctx: int = 4096, max_batch: int = 512, n_seqs: int = 1, device: int = 0,
-                 layer_taps: bool = False) -> "HybridPlan":
+                 layer_taps: bool = False, int8_head: bool = False) -> "HybridPlan":
         assert dtype in ("bfloat16", "float32")
         L = hip.lib()
         if not L.gl3_is_model_dir(path.encode()):
@@ -74,7 +74,7 @@ class HybridPlan:
         opts = hip.ModelDesc()
         opts.struct_size = C.sizeof(hip.ModelDesc)
         opts.ctx, opts.max_batch, opts.n_seqs, opts.device = ctx, max_batch, n_seqs, device
-        opts.flags = (hip.FLAG_F32_COMPUTE if dtype == "float32" else 0) | (hip.FLAG_LAYER_TAPS if layer_taps else 0)
+        opts.flags = (hip.FLAG_F32_COMPUTE if dtype == "float32" else 0) | (hip.FLAG_LAYER_TAPS if layer_taps else 0) | (hip.FLAG_INT8_HEAD if int8_head else 0)
         ptr = C.c_void_p()
         hip.check(L.gl3_load_model_dir(path.encode(), C.byref(opts), C.byref(ptr)))
         return cls(ptr)
@@ -96,6 +96,11 @@ class HybridPlan:
         hip.check(hip.lib().gl3_forward_step(self._ctx, seq, _p(t), t.size, start_pos, _p(w) if w.size else None, w.size,
                                              _p(out) if w.size else None), self._ctx)
         return out
+
+    def score(self, seq: int, tokens, start_pos: int, want, targets=None, top: int = 0) -> dict:
+        """The step, but what comes back of the wanted rows is the log probability and rank of targets[i] (negative: none), the entropy, and the `top`
+        most probable tokens (gl3_forward_score): dict of logprobs, ranks, entropies, top_ids, top_logprobs."""
+        return hip.score_step(self._ctx, seq, tokens, start_pos, want, targets, top)
 
     def layer_rows(self, layer: int, n: int) -> np.ndarray:
         out = np.empty((n, self.dim), np.float32)

@@ -250,6 +250,11 @@ class HipMasterPlan:
         hip.check(hip.lib().gl3_get_kv(self._ctx, layer, pos, _p(k), _p(v)), self._ctx)
         return k, v
 
+    def score(self, tokens, start_pos: int = 0, want=(), targets=None, top: int = 0) -> dict:
+        """The next tokens of sequence 0; of the wanted rows the log probability and rank of targets[i] (negative: none), the entropy and the `top` most
+        probable tokens (gl3_forward_score): dict of logprobs, ranks, entropies, top_ids, top_logprobs."""
+        return hip.score_step(self._ctx, 0, tokens, start_pos, want, targets, top)
+
     def buffer(self, which: int, n: int):
         out = np.empty(n, np.float32)
         hip.check(hip.lib().gl3_get_buffer(self._ctx, which, _p(out), n), self._ctx)

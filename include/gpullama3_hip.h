@@ -323,6 +323,9 @@ enum {
 #define GL3_FLAG_F32_COMPUTE 0x80u /* layer-list family: matrices widened to float32 at upload, every product in true float32 (f32 MFMA);
                                     * default: bfloat16 matrices and activations, float32 accumulation, and float32 for norms, scores,
                                     * softmax, the residual streams and everything inside a recurrence */
+#define GL3_FLAG_INT8_HEAD 0x100u /* layer-list family: the output head in 8-bit integers with one scale per vocabulary row (gl3_quantize_rows at
+                                   * gl3_finalize; a tied head leaves the embedding as it is), its input quantised per token: half the bytes of a
+                                   * bfloat16 head per token, logits within the two roundings to 8 bits.  The GGUF families refuse it */
 
 /* Configuration (J/model/Configuration.java via LlamaModelLoader.java:47-63 / Qwen3ModelLoader.java:48-74)
  * plus the plan-selection knobs the reference reads from system properties
@@ -495,6 +498,13 @@ GL3_API int32_t gl3_forward_prefill_seq(gl3_ctx* ctx, int32_t seq, const int32_t
  * rows run as decode steps and the runs between them as batched prefill. */
 GL3_API int32_t gl3_forward_step(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want,
                                  int32_t n_want, float* logits_out);
+/* Scores of given tokens: the step of gl3_forward_step (same arguments and rules), but the wanted rows' logits stay on the device and what is read
+ * from them comes back (gl3_token_logprobs: definitions and ties).  targets[i]: the token whose log probability wanted row i is asked for (< 0: none
+ * is given, 0 and rank 0); to score a prompt, row i's target is the prompt's token behind it.  targets, logprobs and ranks: all or none (NULL);
+ * entropies may be NULL; top_ids / top_logprobs [n_want][top], 0 <= top <= GL3_LOGPROBS_MAX_TOP. */
+GL3_API int32_t gl3_forward_score(gl3_ctx* ctx, int32_t seq, const int32_t* tokens, int32_t n, int32_t start_pos, const int32_t* want, int32_t n_want,
+                                  const int32_t* targets, int32_t top, float* logprobs, int32_t* ranks, float* entropies, int32_t* top_ids,
+                                  float* top_logprobs);
 /* Sequence slots (n_seqs of them, each with cache rows for ctx positions and its recurrent state): acquire hands out a free slot
  * (GL3_E_STATE when none is free), release gives it back; a released slot's contents are never read again: a sequence that starts at
  * position 0 starts from an empty cache and a zero state whatever the slot held. */
@@ -552,7 +562,7 @@ GL3_API int32_t gl3_probe_peaks(int32_t device, double* hbm_read_gbs, double* hb
 GL3_API int32_t gl3_get_init_ms(gl3_ctx* ctx, double* plan_ms, double* copy_in_ms);
 
 GL3_API void gl3_destroy(gl3_ctx* ctx);
-GL3_API const char* gl3_last_error(gl3_ctx* ctx);  /* ctx may be NULL: last create error */
+GL3_API const char* gl3_last_error(gl3_ctx* ctx);  /* ctx may be NULL: last error without a plan (creating one, operators) of the calling thread */
 
 /* ---- native GGUF loader.  Replaces, for this path, J/tensor/GGUF.java:43-137,217-311 (header,
  * metadata, tensor infos, alignment), the config extraction of LlamaModelLoader.java:47-69 / Qwen3ModelLoader.java:48-79, the

@@ -25,7 +25,12 @@
 //   gl3_run -m model.gguf --ids 1,2,3 [--protocol llama|qwen3] [--bos ID] [-n maxTokens] [-b prefillBatch] [--start-pos P]
 //           [--temperature T] [--top-p P] [--seed S] [--rng l32x64|lcg] [--stop id,id] [--scalar-dot] [--f32-activation]
 // prints "generated: id id ..." (stdout) and the reference's metric lines (stderr).
+//   gl3_run -m model --ids 1,2,3 --score [--top K] [-b prefillBatch] [--f32] [--int8-head] ...
+// generates nothing: id k + 1 is scored behind ids 0 .. k at positions 0 .. k (begin-of-text is the caller's, in --ids).  One line per scored id on stdout,
+// "position id log-probability rank entropy" and with --top K the K most probable ids as "id:log-probability", then "total T, perplexity P over N ids".
+// --int8-head (model folders): GL3_FLAG_INT8_HEAD.
 #include <chrono>
+#include <cmath>
 #include <cstdint>
 #include <cstdio>
 #include <cstdlib>
@@ -85,6 +90,31 @@ static std::vector<int32_t> parse_ids(const char* s) {
     return v;
 }
 
+// Scores of ids 1 .. N - 1 behind the ones in front of them (gl3_forward_score), printed.
+static int score_ids(gl3_ctx* ctx, const std::vector<int32_t>& ids, int top) {
+    const int N = (int)ids.size(), S = N - 1;
+    if (S < 1) { fprintf(stderr, "gl3_run: --score needs two ids at least\n"); return 2; }
+    std::vector<int32_t> want(S), ranks(S), top_ids((size_t)S * top + 1);
+    std::vector<float> lp(S), entropy(S), top_lp((size_t)S * top + 1);
+    for (int i = 0; i < S; ++i) want[i] = i;
+    const double t0 = now_s();
+    if (gl3_forward_score(ctx, 0, ids.data(), S, 0, want.data(), S, ids.data() + 1, top, lp.data(), ranks.data(), entropy.data(), top_ids.data(), top_lp.data()) != GL3_OK) {
+        fprintf(stderr, "gl3_run: %s\n", gl3_last_error(ctx));
+        return 1;
+    }
+    const double t1 = now_s();
+    double total = 0;
+    for (int i = 0; i < S; ++i) {
+        printf("%d %d %.6f %d %.6f", i + 1, ids[i + 1], lp[i], ranks[i], entropy[i]);
+        for (int j = 0; j < top; ++j) printf(" %d:%.6f", top_ids[(size_t)i * top + j], top_lp[(size_t)i * top + j]);
+        printf("\n");
+        total += lp[i];
+    }
+    printf("total %.6f, perplexity %.6f over %d ids\n", total, std::exp(-total / S), S);
+    fprintf(stderr, "scored %d ids in %.1f ms (%.1f tok/s)\n", S, (t1 - t0) * 1e3, S / (t1 - t0 + 1e-12));
+    return 0;
+}
+
 #define CK(call)                                                                                        \
     do {                                                                                                \
         const int32_t r_ = (call);                                                                      \
@@ -95,19 +125,20 @@ static std::vector<int32_t> parse_ids(const char* s) {
 // at position k, all but the last through gl3_forward_prefill in chunks of -b, the last prompt token's logits give the first generated
 // token; -n bounds prompt + generated positions (default 4096); --f32 widens the matrices to float32.
 static int run_model_dir(const std::string& path, const std::vector<int32_t>& prompt, const std::vector<int32_t>& stop, int max_tokens, int batch, float temperature,
-                         float topp, uint64_t seed, const std::string& rng_kind, uint32_t flags) {
+                         float topp, uint64_t seed, const std::string& rng_kind, uint32_t flags, bool score, int top) {
     gl3_ctx* ctx = nullptr;
     gl3_model_desc opts{};
     opts.struct_size = sizeof(opts);
     opts.ctx = max_tokens > 0 ? max_tokens : 0;
     opts.max_batch = batch > 1 ? batch : 512;
-    opts.flags = flags & GL3_FLAG_F32_COMPUTE;
+    opts.flags = flags & (GL3_FLAG_F32_COMPUTE | GL3_FLAG_INT8_HEAD);
     if (gl3_load_model_dir(path.c_str(), &opts, &ctx) != GL3_OK) { fprintf(stderr, "gl3_run: %s\n", gl3_last_error(nullptr)); return 1; }
     gl3_model_desc d{};
     gl3_get_model_desc(ctx, &d);
     for (int32_t t : prompt) if (t < 0 || t >= d.vocab) { fprintf(stderr, "gl3_run: prompt id %d outside the vocabulary\n", t); gl3_destroy(ctx); return 2; }
     const int N = (int)prompt.size(), limit = d.ctx;
     if (N > limit) { fprintf(stderr, "gl3_run: the prompt is longer than the context (%d)\n", limit); gl3_destroy(ctx); return 2; }
+    if (score) { const int rc = score_ids(ctx, prompt, top); gl3_destroy(ctx); return rc; }
     const std::set<int32_t> stop_set(stop.begin(), stop.end());
     JavaRandom lcg(seed);
     L32X64MixRandom mix(seed);
@@ -139,7 +170,8 @@ static int run_model_dir(const std::string& path, const std::vector<int32_t>& pr
 int main(int argc, char** argv) {
     std::string path, protocol, rng_kind = "l32x64";
     std::vector<int32_t> prompt, stop;
-    int max_tokens = 0, batch = 1, start_pos = 0, bos = -1;
+    int max_tokens = 0, batch = 1, start_pos = 0, bos = -1, top = 0;
+    bool score = false;
     float temperature = 0.f, topp = 0.95f;
     uint64_t seed = 1234;                                  // the reference's default (Options.java)
     uint32_t flags = 0;
@@ -161,11 +193,15 @@ int main(int argc, char** argv) {
         else if (a == "--scalar-dot") flags |= GL3_FLAG_SCALAR_DOT;
         else if (a == "--f32-activation") flags |= GL3_FLAG_F32_ACTIVATION;
         else if (a == "--f32") flags |= GL3_FLAG_F32_COMPUTE;
+        else if (a == "--int8-head") flags |= GL3_FLAG_INT8_HEAD;
+        else if (a == "--score") score = true;
+        else if (a == "--top") top = atoi(val());
         else { fprintf(stderr, "gl3_run: unknown argument %s (see the header of tools/gl3_run.cpp)\n", a.c_str()); return 2; }
     }
     if (path.empty() || prompt.empty()) { fprintf(stderr, "gl3_run: -m model.gguf and --ids a,b,c are required\n"); return 2; }
 
-    if (gl3_is_model_dir(path.c_str())) return run_model_dir(path, prompt, stop, max_tokens, batch, temperature, topp, seed, rng_kind, flags);
+    if (top < 0 || top > GL3_LOGPROBS_MAX_TOP) { fprintf(stderr, "gl3_run: --top 0 .. %d\n", GL3_LOGPROBS_MAX_TOP); return 2; }
+    if (gl3_is_model_dir(path.c_str())) return run_model_dir(path, prompt, stop, max_tokens, batch, temperature, topp, seed, rng_kind, flags, score, top);
 
     gl3_gguf* g = nullptr;
     gl3_model_desc d{};
@@ -194,6 +230,7 @@ int main(int argc, char** argv) {
         if (gl3_gguf_open(path.c_str(), &g2) == GL3_OK) { live.ctx = opts.ctx; gl3_gguf_model_desc(g2, &live, nullptr); gl3_gguf_close(g2); }
     }
     const int ctx_len = live.ctx > 0 ? live.ctx : (opts.ctx > 0 ? opts.ctx : 4096);
+    if (score) { const int rc = score_ids(ctx, prompt, top); gl3_destroy(ctx); return rc; }
     const int actual_max = max_tokens > 0 && max_tokens < ctx_len ? max_tokens : ctx_len;
     const std::set<int32_t> stop_set(stop.begin(), stop.end());
     JavaRandom lcg(seed);
