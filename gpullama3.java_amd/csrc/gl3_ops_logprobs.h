@@ -3,8 +3,8 @@
 // One pass over the logits.  A wavefront keeps, for what it has seen of a row: the largest logit m (one value, all lanes), per lane
 // s = sum e^(x - m) and t = sum e^(x - m) (x - m) (a new maximum scales both, once per batch of 32 logits a lane at most), how many logits stand
 // in front of the given one, and the best 64 tokens, one a lane, sorted.  A batch touches the list only if one of its logits reaches the smallest
-// of the `top` kept (lo): such logits are collected in LDS, 64 at a time are sorted (bitonic network) and merged.  lo starts as the top-th largest
-// of the first batch's 64 lane maxima, so that batch adds about `top` candidates and not all it holds.
+// of the `top` kept (lo): such logits are collected in LDS, 64 at a time are sorted (bitonic network) and merged.  lo comes from the
+// largest logits of the lanes (behind batch 1, 2, 4, ...), so the first batch adds about `top` candidates and not all it holds.
 // With P = sum p (x - m) = t / s:  lse = m + ln s,  logprob = (x_t - m) - ln s,  entropy = ln s - P: both terms >= 0, nothing cancels.
 #pragma once
 #include "gl3_ops_int8.h"          // element types
@@ -89,13 +89,21 @@ struct OpTop {
     float mine;              // the largest logit this lane has seen
     int seen, next;          // batches; lo is put up behind batch 1, 2, 4, ...
     __device__ __forceinline__ void init() { key = 0; lo = -3.402823466e38f; n = 0; any_key = false; mine = -INFINITY; seen = 0; next = 1; }
-    // at least `top` lanes have seen a logit as large as the top-th largest of what the lanes have seen at most: nothing below it can enter
-    __device__ __forceinline__ void batch_max(float mx, int top) {
+    static __device__ __forceinline__ float logit(uint32_t ord) { return __uint_as_float(ord >> 31 ? ord & 0x7fffffffu : ~ord); }
+    // Nothing below the top-th largest of what this wavefront's lanes have seen at most can enter: `top` of them have seen as much.  Nor below what a quarter of
+    // `top` lanes of each of the four wavefronts have seen.  (All wavefronts come here together.)
+    __device__ __forceinline__ void batch_max(float mx, int top, uint32_t (*bound)[OP_LP_WAVES], int wave) {
         mine = fmaxf(mine, mx);
         if (++seen < next) return;
         next = 2 * seen;
-        const uint32_t k = __float_as_uint(mine), kth = __builtin_amdgcn_readlane(op_sort64<true>(k >> 31 ? ~k : k | 0x80000000u), top - 1);
-        lo = fmaxf(lo, __uint_as_float(kth >> 31 ? kth & 0x7fffffffu : ~kth));
+        const uint32_t k = __float_as_uint(mine), ord = op_sort64<true>(k >> 31 ? ~k : k | 0x80000000u);
+        uint32_t* b = bound[__builtin_ctz(seen) & 1];          // (the last bounds may still be read)
+        if ((threadIdx.x & 63) == 0) b[wave] = __builtin_amdgcn_readlane(ord, (top + OP_LP_WAVES - 1) / OP_LP_WAVES - 1);
+        __syncthreads();
+        uint32_t least = b[0];
+#pragma unroll
+        for (int w = 1; w < OP_LP_WAVES; ++w) least = min(least, b[w]);
+        lo = fmaxf(lo, fmaxf(logit(__builtin_amdgcn_readlane(ord, top - 1)), logit(__builtin_amdgcn_readfirstlane(least))));
     }
     // 64 of the collected candidates, or what is left of them, into the list
     __device__ __forceinline__ void merge(uint64_t* buf, int top, int lane) {
@@ -166,6 +174,8 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 5) void op_logprobs_kernel(co
     constexpr int V = OpVec<T>::N, NT = OP_LP_THREADS;
     __shared__ uint64_t buf_s[TOP ? OP_LP_WAVES : 1][TOP ? 64 * V + 64 : 1];
     __shared__ OpSums sums_s[OP_LP_WAVES];
+    __shared__ uint32_t bound_s[2][OP_LP_WAVES];
+    __shared__ int got_s[OP_LP_WAVES];          // a wavefront's candidates that are in no list, and whether it has a list (at its buffer's 64)
     __shared__ int front_s[OP_LP_WAVES];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int64_t row = row0 + blockIdx.y;
@@ -223,7 +233,7 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 5) void op_logprobs_kernel(co
             }
         }
         if constexpr (TOP) {
-            best.batch_max(mx, o.top);
+            best.batch_max(mx, o.top, bound_s, wave);
             int i0 = 0;
             while (i0 < U && __any(mx >= best.lo)) {          // from vector i0 on: until 64 are together
                 int next = U;
@@ -277,12 +287,15 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 5) void op_logprobs_kernel(co
         u[0] = fmaf(p, fmaxf(d, -200.f), u[0]);
         front += __popcll(__ballot(in && (v > xt || (v == xt && id < t))));
         if constexpr (TOP) {
-            if (best.n) best.merge(buf, o.top, lane);
             // ids of the head are lower than the list's: equal to its last one is enough
             best.collect(buf, v, id, in && v > -INFINITY);
         }
     }
-    if constexpr (TOP) while (best.n) best.merge(buf, o.top, lane);
+    if constexpr (TOP) {
+        while (best.n >= 64) best.merge(buf, o.top, lane);
+        if (best.any_key) buf[64 + lane] = best.key;
+        if (lane == 0) got_s[wave] = best.n | (best.any_key ? 256 : 0);
+    }
     // logits of t's own vector that stand in front of it with the same value
     if (given && t >= head && t < head + nv * V && (t - head) / V >= v0 && (t - head) / V < v1 && wave == 0) {
         const int first = head + (t - head) / V * V;
@@ -290,7 +303,6 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 5) void op_logprobs_kernel(co
     }
     const OpSums mine{m, op_wave_sum(s[0] + s[1]), op_wave_sum(u[0] + u[1])};
     if (lane == 0) { sums_s[wave] = mine; front_s[wave] = front; }
-    if constexpr (TOP) if (wave) buf[lane] = best.key;
     __syncthreads();
     if (wave) return;
     OpSums all = mine;
@@ -298,7 +310,20 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 5) void op_logprobs_kernel(co
     for (int w = 1; w < OP_LP_WAVES; ++w) {
         all = op_join(all, sums_s[w]);
         front += front_s[w];
-        if constexpr (TOP) best.key = op_merge64(best.key, buf_s[w][63 - lane]);
+    }
+    if constexpr (TOP) {          // one list of all: the candidates 64 at a time, then the lists there are
+        int end[OP_LP_WAVES], n = 0;
+#pragma unroll
+        for (int w = 0; w < OP_LP_WAVES; ++w) end[w] = n += got_s[w] & 255;
+        uint64_t key = 0;
+        for (int i = 0; i < n; i += 64) {
+            const int at = i + lane, w = (at >= end[0]) + (at >= end[1]) + (at >= end[2]);
+            const uint64_t c = at < n ? buf_s[w][at - (w == 0 ? 0 : w == 1 ? end[0] : w == 2 ? end[1] : end[2])] : 0;
+            key = i == 0 ? op_sort64<true>(c) : op_merge64(key, op_sort64<false>(c));
+        }
+#pragma unroll
+        for (int w = 0; w < OP_LP_WAVES; ++w) if (got_s[w] & 256) key = op_merge64(key, buf_s[w][64 + 63 - lane]);
+        best.key = key;
     }
     if (gridDim.x == 1) op_row_results(o, row, vocab, xt, all, front, best.key, lane);
     else {
