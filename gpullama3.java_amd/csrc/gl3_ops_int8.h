@@ -128,6 +128,11 @@ static __global__ __launch_bounds__(1024) void op_quantize_long_kernel(const T* 
 
 // ---- products -------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float op_result(int acc, float as, float ws) { return ((float)acc * as) * ws; }
+// Results go past the caches: in them they push out weights on their way (64 tokens, 151936 x 2560 float32, us: through / past them 100 / 86; none stored 81).
+template <typename TY> __device__ __forceinline__ void op_store_past(TY* p, TY v) {
+    if constexpr (sizeof(TY) == 4) __builtin_nontemporal_store(v, p);
+    else __builtin_nontemporal_store(__builtin_bit_cast(uint16_t, v), reinterpret_cast<uint16_t*>(p));
+}
 template <typename TY> struct OpProductArgs {
     const int8_t* a; int64_t lda; const float* as;
     const int8_t* w; int64_t ldw; const float* ws; const float* bias;
@@ -414,127 +419,10 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
                         const int row = mb + i * 32 + 8 * g + r;          // (of lanes 0 .. 31)
                         const float x = op_result(acc[i][j][4 * g + r], s4[r], w_);
                         if (ALL || (row + 4 * kh < p.m && n0 + cn < p.n))
-                            *reinterpret_cast<TY*>(reinterpret_cast<uint8_t*>(p.y + row * p.ldy + nb + j * 32) + lo) = op_cast<TY>(biased ? x + b_ : x);
+                            op_store_past(reinterpret_cast<TY*>(reinterpret_cast<uint8_t*>(p.y + row * p.ldy + nb + j * 32) + lo), op_cast<TY>(biased ? x + b_ : x));
                     }
                 }
         }
     };
     if (whole) store(std::true_type{}); else store(std::false_type{});
-}
-
-// A few tokens (m <= BM) and many channels: what the weights take to leave memory is the time, so their stream must not stop.  Workgroup b has the channel
-// tiles [nt b / grid, nt (b + 1) / grid) one behind the other, as one long row of stages: the next tile's first stages are on their way while one ends (a
-// workgroup per tile fills and drains its rings for every tile).  Rings, swizzle and barriers as above; a wavefront has one 32 x 32 tile.  The channels'
-// scales of all its tiles wait in LDS, the tokens' in registers.  (Stores are counted with the loads: the barrier behind a tile's results waits for them too.)
-constexpr int OP_FLOW_WGS = 512;
-template <int BN> struct OpFlow { static constexpr int TILES = (1 << 18) / BN / OP_FLOW_WGS; };          // most tiles of a workgroup: OP_MAX_N channels a launch
-template <typename TY, int BM, int BN, int WM, int WN, int SA, int SW>
-static __global__ __launch_bounds__(WM * WN * 64) void op_flow_kernel(OpProductArgs<TY> p, int nt) {
-    constexpr int NW = WM * WN;
-    constexpr int PA = BM / 8, PW = BN / 8, NPA = PA / NW, NPW = PW / NW, NP = NPA + NPW;
-    constexpr int SZA = BM * 128, SZW = BN * 128, OW = SA * SZA, SCALES = OpFlow<BN>::TILES * BN;
-    static_assert(SW >= SA + 1 && SA >= 2 && WM * 32 == BM && WN * 32 == BN && NPA * NW == PA && NPW * NW == PW, "tile layout");
-    static_assert(SA * SZA + SW * SZW + SCALES * 8 <= 80 * 1024, "two workgroups share a CU");
-    __shared__ __attribute__((aligned(1024))) uint8_t smem[SA * SZA + SW * SZW];
-    __shared__ float lws[SCALES], lb[SCALES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN, r32 = lane & 31, kh = lane >> 5;
-    const int t0 = (int)((int64_t)nt * blockIdx.x / gridDim.x), t1 = (int)((int64_t)nt * (blockIdx.x + 1) / gridDim.x), n_it = p.kp / 128, total = (t1 - t0) * n_it;
-    for (int i = tid; i < (t1 - t0) * BN; i += NW * 64) {
-        const int c = min(t0 * BN + i, p.n - 1);
-        lws[i] = p.ws[c];
-        lb[i] = p.bias ? p.bias[c] : 0.f;
-    }
-    float as[16];
-#pragma unroll
-    for (int r = 0; r < 16; ++r) as[r] = p.as[min(wm * 32 + 8 * (r >> 2) + 4 * kh + (r & 3), p.m - 1)];
-    // this wavefront's pieces; the next stage to load of either operand
-    uint32_t offa[NPA], offw[NPW];
-    int pa[NPA], pw[NPW];
-    const int8_t *la = p.a, *lw = p.w + (int64_t)t0 * BN * p.ldw;
-    int ka = 0, kw = 0, tw = t0;
-#pragma unroll
-    for (int u = 0; u < NPA; ++u) {
-        const int q = wave + NW * u, row = 8 * q + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
-        pa[u] = q * 1024;
-        offa[u] = (uint32_t)min(row, p.m - 1) * (uint32_t)p.lda + 16 * c;
-    }
-    auto rows_w = [&]() {          // of tile tw (rows past the end repeat the last one)
-#pragma unroll
-        for (int u = 0; u < NPW; ++u) {
-            const int q = wave + NW * u, row = 8 * q + (lane >> 3), c = (lane & 7) ^ ((row >> 1) & 7);
-            pw[u] = OW + q * 1024;
-            offw[u] = (uint32_t)(min(tw * BN + row, p.n - 1) - tw * BN) * (uint32_t)p.ldw + 16 * c;
-        }
-    };
-    rows_w();
-    int slot_a = 0, slot_w = 0;          // where they go
-    auto issue_a = [&]() {
-#pragma unroll
-        for (int u = 0; u < NPA; ++u) op_dma16(la + offa[u], smem + slot_a * SZA + pa[u]);
-        la += 128;
-        if (++ka == n_it) { ka = 0; la = p.a; }
-        if (++slot_a == SA) slot_a = 0;
-    };
-    auto issue_w = [&]() {
-#pragma unroll
-        for (int u = 0; u < NPW; ++u) op_dma16(lw + offw[u], smem + slot_w * SZW + pw[u]);
-        lw += 128;
-        if (++kw == n_it) { kw = 0; ++tw; lw = p.w + (int64_t)tw * BN * p.ldw; rows_w(); }
-        if (++slot_w == SW) slot_w = 0;
-    };
-    op_v16i acc;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0;
-    uint32_t ca[4];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) ca[q] = ((2 * q + kh) ^ ((r32 >> 1) & 7)) * 16;
-    const uint32_t aw = (wm * 32 + r32) * 128, ww = OW + (wn * 32 + r32) * 128;
-    // stage s: behind barrier s a's stage s + SA starts, w's stage s + SW in front of barrier s + 1
-    constexpr int LEFT = (SA - 2) * NP + NPW;
-#pragma unroll
-    for (int s = -SW; s < 0; ++s) {
-        if (s + SA >= 0 && s + SA < total) issue_a();
-        if (s < -1 && s + SW < total) issue_w();
-    }
-    op_wait_barrier<0>();          // (and the scales are in LDS)
-    int sa = 0, sw = 0, k = 0, tile = t0;
-    op_v4i fa[2], fw[2];
-    auto rd = [&](int set, int q) {
-        fa[set] = *reinterpret_cast<const op_v4i*>(smem + sa * SZA + aw + ca[q]);
-        fw[set] = *reinterpret_cast<const op_v4i*>(smem + sw * SZW + ww + ca[q]);
-    };
-    auto mm = [&](int set) { acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(fa[set], fw[set], acc, 0, 0, 0); };
-    rd(0, 0);
-    for (int g = 0; g < total; ++g) {
-        rd(1, 1); mm(0);
-        if (g - 1 + SW < total) issue_w();
-        rd(0, 2); mm(1);
-        rd(1, 3); mm(0);
-        __builtin_amdgcn_s_waitcnt(0xc07f);
-        if (g < total - SW) op_wait_barrier<LEFT>(); else op_wait_barrier<0>();
-        if (++sa == SA) sa = 0;
-        if (++sw == SW) sw = 0;
-        if (g + 1 < total) rd(0, 0);
-        mm(1);
-        if (g + SA < total) issue_a();
-        if (++k == n_it) {          // the tile is through: lane holds channel lane % 32 and tokens 8 (r / 4) + 4 (lane / 32) + r % 4
-            const int c = wn * 32 + r32, n = tile * BN + c;
-            const float w_ = lws[(tile - t0) * BN + c], b_ = lb[(tile - t0) * BN + c];
-            if (n < p.n) {
-                TY* y = p.y + (int64_t)(wm * 32 + 4 * kh) * p.ldy + n;
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int row = 8 * (r >> 2) + (r & 3);
-                    if (wm * 32 + 4 * kh + row < p.m) {
-                        const float x = op_result(acc[r], as[r], w_);
-                        y[(int64_t)row * p.ldy] = op_cast<TY>(p.bias ? x + b_ : x);
-                    }
-                }
-            }
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[r] = 0;
-            k = 0;
-            ++tile;
-        }
-    }
 }
