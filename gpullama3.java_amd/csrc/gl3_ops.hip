@@ -38,7 +38,7 @@ void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32
 uint64_t op_product_workspace(int64_t, int64_t, int32_t) { return 0; }
 
 // Which tile: the one with the least estimated time.  A stage of a BM x BN tile takes a CU 0.00164 (BM + BN) us for its operands' bytes + 0.0000101 BM BN us for its
-// MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 64 x 64 0.25), a tile 3 us and its results' bytes at 20 GB/s besides.  256 CUs take the
+// MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 64 x 64 0.25), a tile 3 us and its results' bytes at 37 GB/s besides.  256 CUs take the
 // workgroups in rounds; two workgroups of a small tile share a CU.
 enum { OP_T256x256, OP_T128x256, OP_T256x128, OP_T128x128, OP_T64x128, OP_T64x64, OP_T_COUNT };
 static const struct { int bm, bn, share; } OP_TILES[OP_T_COUNT] = {{256, 256, 1}, {128, 256, 1}, {256, 128, 1}, {128, 128, 2}, {64, 128, 2}, {64, 64, 2}};
@@ -47,7 +47,7 @@ static int op_ring_pick(int m, int n, int kp, int size, double* us_out) {
     double least = 1e300;
     for (int t = 0; t < OP_T_COUNT; ++t) {
         const int bm = OP_TILES[t].bm, bn = OP_TILES[t].bn, slots = 256 * OP_TILES[t].share;
-        const double one = kp / 128 * (0.00164 * (bm + bn) + 0.0000101 * bm * bn) + 3.0 + (double)bm * bn * size / 20e3;
+        const double one = kp / 128 * (0.00164 * (bm + bn) + 0.0000101 * bm * bn) + 3.0 + (double)bm * bn * size / 37e3;
         const int64_t tiles = op_cdiv(m, bm) * op_cdiv(n, bn), rest = tiles % slots;
         const double us = (double)(tiles / slots * OP_TILES[t].share + (rest == 0 ? 0 : rest <= 256 ? 1 : 2)) * one;
         if (us < least) { least = us; best = t; }
@@ -63,7 +63,7 @@ static void op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p) {
 template <typename TY>
 static void op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile) {
     switch (tile) {
-        case OP_T256x256: op_ring_launch<TY, 256, 256, 2, 4, 2, 3>(s, p); break;
+        case OP_T256x256: op_ring_launch<TY, 256, 256, 4, 2, 2, 3>(s, p); break;
         case OP_T128x256: op_ring_launch<TY, 128, 256, 2, 4, 2, 4>(s, p); break;
         case OP_T256x128: op_ring_launch<TY, 256, 128, 4, 2, 3, 4>(s, p); break;
         case OP_T128x128: op_ring_launch<TY, 128, 128, 2, 2, 2, 3>(s, p); break;

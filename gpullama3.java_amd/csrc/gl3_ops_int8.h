@@ -405,24 +405,25 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
     const uint32_t lo = ((uint32_t)(4 * kh) * (uint32_t)p.ldy + r32) * (uint32_t)sizeof(TY);
     auto store = [&](auto all) {
         constexpr bool ALL = decltype(all)::value;
+        float w_[TN], b_[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int cn = wn * (BN / WN) + j * 32 + r32;
-            const float w_ = lws[cn], b_ = lb[cn];
+        for (int j = 0; j < TN; ++j) { const int c = wn * (BN / WN) + j * 32 + r32; w_[j] = lws[c]; b_[j] = lb[c]; }
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float* s4 = las + wm * (BM / WM) + i * 32 + 8 * g + 4 * kh;
+            for (int g = 0; g < 4; ++g) {
+                const float* s4 = las + wm * (BM / WM) + i * 32 + 8 * g + 4 * kh;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int row = mb + i * 32 + 8 * g + r;          // (of lanes 0 .. 31)
-                        const float x = op_result(acc[i][j][4 * g + r], s4[r], w_);
-                        if (ALL || (row + 4 * kh < p.m && n0 + cn < p.n))
-                            op_store_past(reinterpret_cast<TY*>(reinterpret_cast<uint8_t*>(p.y + row * p.ldy + nb + j * 32) + lo), op_cast<TY>(biased ? x + b_ : x));
+                for (int r = 0; r < 4; ++r) {
+                    const int row = mb + i * 32 + 8 * g + r;          // (of lanes 0 .. 31)
+                    uint8_t* y = reinterpret_cast<uint8_t*>(p.y + row * p.ldy + nb);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {          // (a row's columns one behind the other: with the rows inside, 13.4 us a float32 tile of 256 x 256 instead of 5)
+                        const float x = op_result(acc[i][j][4 * g + r], s4[r], w_[j]);
+                        if (ALL || (row + 4 * kh < p.m && nb + j * 32 + r32 < p.n)) op_store_past(reinterpret_cast<TY*>(y + j * 32 * sizeof(TY) + lo), op_cast<TY>(biased ? x + b_[j] : x));
                     }
                 }
-        }
+            }
     };
     if (whole) store(std::true_type{}); else store(std::false_type{});
 }
