@@ -24,10 +24,10 @@
 #include "gl3_moe_kernels.h"
 #include "gl3_hy_dispatch.h"
 
+#include "gl3_create_err.h"
+
 using namespace gl3;
 
-static thread_local std::string g_create_err;          // of the calling thread: operators are called from several at once
-void gl3_set_create_error(const char* msg) { try { g_create_err = msg ? msg : ""; } catch (...) { g_create_err.clear(); } }
 
 static double now_ms() {
     return std::chrono::duration<double, std::milli>(std::chrono::steady_clock::now().time_since_epoch()).count();
@@ -571,17 +571,17 @@ int32_t gl3_debug_sumsq(int32_t device, const float* x, int32_t n, float* out) {
 
 const char* gl3_version(void) { return "gpullama3-hip 0.1 (gfx950)"; }
 
-const char* gl3_last_error(gl3_ctx* ctx) { return ctx ? ctx->err.c_str() : g_create_err.c_str(); }
+const char* gl3_last_error(gl3_ctx* ctx) { return ctx ? ctx->err.c_str() : create_error(); }
 
 int32_t gl3_create(const gl3_model_desc* desc, gl3_ctx** out) {
-    if (!desc || !out) { g_create_err = "null argument"; return GL3_E_ARG; }
-    if (desc->struct_size != sizeof(gl3_model_desc)) { g_create_err = "gl3_model_desc.struct_size mismatch"; return GL3_E_ARG; }
-    if (desc->arch == GL3_ARCH_NODITAR) return gl3_hy_create(desc, out, g_create_err);
+    if (!desc || !out) { gl3_set_create_error("null argument"); return GL3_E_ARG; }
+    if (desc->struct_size != sizeof(gl3_model_desc)) { gl3_set_create_error("gl3_model_desc.struct_size mismatch"); return GL3_E_ARG; }
+    if (desc->arch == GL3_ARCH_NODITAR) { const int32_t r = gl3_hy_create(desc, out, g_create_err); if (r != GL3_OK) publish_create_error(); return r; }
     gl3_ctx* ctx = new gl3_ctx();
     ctx->d = *desc;
     ctx->n_seqs = desc->n_seqs < 1 ? 1 : desc->n_seqs;
     const gl3_model_desc& d = ctx->d;
-    auto bail = [&](int32_t code, const std::string& msg) { g_create_err = msg.empty() ? ctx->err : msg; gl3_destroy(ctx); return code; };
+    auto bail = [&](int32_t code, const std::string& msg) { gl3_set_create_error(msg.empty() ? ctx->err.c_str() : msg.c_str()); gl3_destroy(ctx); return code; };
     const double t0 = now_ms();
     if (d.arch != GL3_ARCH_LLAMA && d.arch != GL3_ARCH_QWEN3 && d.arch != GL3_ARCH_QWEN2 && d.arch != GL3_ARCH_GRANITE && d.arch != GL3_ARCH_PHI3 &&
         d.arch != GL3_ARCH_QWEN2MOE)

@@ -3,10 +3,9 @@
 // the GGUF families; a host links against either.
 #include <string>
 
+#include "gl3_create_err.h"
 #include "gl3_hy_dispatch.h"
 
-static thread_local std::string g_create_err;          // of the calling thread: operators are called from several at once
-void gl3_set_create_error(const char* msg) { try { g_create_err = msg ? msg : ""; } catch (...) { g_create_err.clear(); } }
 int32_t gl3_tp_check(gl3_ctx*) { return GL3_OK; }          // no tensor-parallel transport in this build
 
 #define LEAN_CTX(c) do { if (!(c)) return GL3_E_ARG; if (!(c)->hy) return GL3_E_UNSUPPORTED; } while (0)
@@ -14,13 +13,15 @@ int32_t gl3_tp_check(gl3_ctx*) { return GL3_OK; }          // no tensor-parallel
 extern "C" {
 
 const char* gl3_version(void) { return "gpullama3-hip (layer-list family only)"; }
-const char* gl3_last_error(gl3_ctx* ctx) { return ctx ? ctx->err.c_str() : g_create_err.c_str(); }
+const char* gl3_last_error(gl3_ctx* ctx) { return ctx ? ctx->err.c_str() : create_error(); }
 
 int32_t gl3_create(const gl3_model_desc* desc, gl3_ctx** out) {
-    if (!desc || !out) { g_create_err = "null argument"; return GL3_E_ARG; }
-    if (desc->struct_size != sizeof(gl3_model_desc)) { g_create_err = "gl3_model_desc.struct_size mismatch"; return GL3_E_ARG; }
-    if (desc->arch != GL3_ARCH_NODITAR) { g_create_err = "this build carries the layer-list family only"; return GL3_E_UNSUPPORTED; }
-    return gl3_hy_create(desc, out, g_create_err);
+    if (!desc || !out) { gl3_set_create_error("null argument"); return GL3_E_ARG; }
+    if (desc->struct_size != sizeof(gl3_model_desc)) { gl3_set_create_error("gl3_model_desc.struct_size mismatch"); return GL3_E_ARG; }
+    if (desc->arch != GL3_ARCH_NODITAR) { gl3_set_create_error("this build carries the layer-list family only"); return GL3_E_UNSUPPORTED; }
+    const int32_t r = gl3_hy_create(desc, out, g_create_err);
+    if (r != GL3_OK) publish_create_error();
+    return r;
 }
 
 void gl3_destroy(gl3_ctx* ctx) {
@@ -84,7 +85,7 @@ int32_t gl3_get_model_desc(gl3_ctx* ctx, gl3_model_desc* desc) {
     return GL3_OK;
 }
 int32_t gl3_load_gguf(const char*, const gl3_model_desc*, gl3_ctx**) {
-    g_create_err = "this build carries the layer-list family only: GGUF models need the whole library (make -C gpullama3.java_amd/csrc)";
+    gl3_set_create_error("this build carries the layer-list family only: GGUF models need the whole library (make -C gpullama3.java_amd/csrc)");
     return GL3_E_UNSUPPORTED;
 }
 int32_t gl3_profile_hybrid_gemm(int32_t device, int32_t f32, int32_t rows, int32_t k, int32_t m, int32_t glu, int32_t iters, double* out_us) {

@@ -191,6 +191,7 @@ int32_t gl3_hy_create(const gl3_model_desc* desc, gl3_ctx** out, std::string& er
     for (int l = 0; l < desc->n_layers && desc->streams > 0; ++l)
         if (desc->layer_descs[l].experts > 0) { err = "layer-list family: a mixture of experts needs the plain residual (streams = 0)"; return GL3_E_ARG; }
     if (desc->dim < 1 || desc->vocab < 1 || desc->ctx < 1) { err = "layer-list family: dim, vocab and ctx must be positive"; return GL3_E_ARG; }
+    if ((desc->flags & GL3_FLAG_INT8_HEAD) && (desc->dim > GL3_INT8_MAX_K || desc->vocab > 1 << 26)) { err = "layer-list family: GL3_FLAG_INT8_HEAD takes dim <= GL3_INT8_MAX_K and vocab <= 2^26"; return GL3_E_ARG; }
     if (desc->weight_type != GL3_TYPE_BF16 && desc->weight_type != GL3_TYPE_F32) { err = "layer-list family: weight_type must be GL3_TYPE_BF16 (or GL3_TYPE_F32)"; return GL3_E_UNSUPPORTED; }
     if (desc->tp_size > 1) { err = "layer-list family: tensor parallelism is not built"; return GL3_E_UNSUPPORTED; }
     if (desc->post_norms && (desc->streams > 0 || desc->depth_mix || desc->parallel_block)) { err = "layer-list family: post norms need the plain residual without depth average and parallel block"; return GL3_E_ARG; }
@@ -934,9 +935,9 @@ int32_t gl3_hy_finalize(gl3_ctx* ctx) {
         h->head_ldq = op_code_ld(W);
         uint64_t ws = 0;
         for (int m = 1; m <= h->want_cap; ++m) ws = std::max(ws, op_linear_workspace(m, V, W));
-        HY_HIP(hipMalloc((void**)&h->head_q, (size_t)V * h->head_ldq));
-        HY_HIP(hipMalloc((void**)&h->head_s, (size_t)V * 4));
-        HY_HIP(hipMalloc(&h->head_ws, std::max<uint64_t>(ws, 16)));
+        if (!h->head_q) HY_HIP(hipMalloc((void**)&h->head_q, (size_t)V * h->head_ldq));
+        if (!h->head_s) HY_HIP(hipMalloc((void**)&h->head_s, (size_t)V * 4));
+        if (!h->head_ws) HY_HIP(hipMalloc(&h->head_ws, std::max<uint64_t>(ws, 16)));
         op_quantize(ctx->stream, h->head.w, h->f32 ? GL3_TYPE_F32 : GL3_TYPE_BF16, V, W, h->head.ld, h->head_q, h->head_ldq, h->head_s);
         HY_HIP(hipGetLastError());
         HY_HIP(hipStreamSynchronize(ctx->stream));

@@ -230,6 +230,6 @@ def score_step(ctx, seq, tokens, start_pos, want, targets, top):
     if g is not None and g.shape != w.shape:
         raise Gl3Error(E_ARG, "one target per wanted row")
     r = {"logprobs": None if g is None else np.empty(w.size, np.float32), "ranks": None if g is None else np.empty(w.size, np.int32), "entropies": np.empty(w.size, np.float32),
-         "top_ids": np.empty((w.size, top), np.int32) if top > 0 else None, "top_logprobs": np.empty((w.size, top), np.float32) if top > 0 else None}
+         "top_ids": np.empty((w.size, top), np.int32) if 0 < top <= 64 else None, "top_logprobs": np.empty((w.size, top), np.float32) if 0 < top <= 64 else None}
     check(lib().gl3_forward_score(ctx, seq, p(t), t.size, start_pos, p(w), w.size, p(g), top, p(r["logprobs"]), p(r["ranks"]), p(r["entropies"]), p(r["top_ids"]), p(r["top_logprobs"])), ctx)
     return r

@@ -128,3 +128,36 @@ def test_errors_belong_to_the_thread(hip):
         t.join()
     assert all(len(v) == 1 for v in seen.values()) and len(seen) == 4
     assert all((b"top" in next(iter(v))) == bool(i % 2) for i, v in seen.items())
+
+
+@pytest.mark.parametrize("i", range(9))
+def test_strides_beyond_the_documented_ones(hip, i):
+    name, make, kw = [("gl3_int8_matmul", matmul, dict(ldw=(1 << 23) + 16)), ("gl3_int8_matmul", matmul, dict(lda=(1 << 23) + 16)), ("gl3_int8_matmul", matmul, dict(ldy=(1 << 26) + 1)),
+                      ("gl3_int8_linear", linear, dict(ldw=(1 << 23) + 16)), ("gl3_int8_linear", linear, dict(ldy=(1 << 26) + 1)), ("gl3_int8_linear", linear, dict(ldx=1 << 62)),
+                      ("gl3_token_logprobs", logprobs, dict(vocab=(1 << 30) + 1, ld=(1 << 30) + 1)), ("gl3_token_logprobs", logprobs, dict(ld=1 << 62)),
+                      ("gl3_token_logprobs", logprobs, dict(vocab=128256, ld=128256, bytes=100))][i]
+    assert getattr(hip.lib(), name)(*make(**kw)) == hip.E_ARG, (name, kw)
+
+
+def test_a_thread_without_an_error_reads_the_newest(hip):
+    """A plan that cannot be created in one thread, its message read in another that has none of its own."""
+    import threading
+    L = hip.lib()
+    out = C.c_void_p()
+    assert L.gl3_create(None, C.byref(out)) == hip.E_ARG
+    seen = []
+    t = threading.Thread(target=lambda: seen.append(L.gl3_last_error(None)))
+    t.start()
+    t.join()
+    assert seen == [b"null argument"] == [L.gl3_last_error(None)]
+
+
+@pytest.mark.parametrize("over", [dict(dim=131072), dict(vocab=(1 << 26) + 1)])
+def test_an_int8_head_of_what_it_cannot_hold(hip, over):
+    """Refused before anything is allocated."""
+    d = hip.ModelDesc()
+    layer = hip.LayerDesc()
+    for k, v in dict(dict(struct_size=C.sizeof(d), arch=hip.ARCH_NODITAR, dim=64, vocab=100, ctx=16, n_layers=1, weight_type=30, flags=hip.FLAG_INT8_HEAD, layer_descs=C.pointer(layer)), **over).items():
+        setattr(d, k, v)
+    out = C.c_void_p()
+    assert hip.lib().gl3_create(C.byref(d), C.byref(out)) == hip.E_ARG and b"INT8_HEAD" in hip.lib().gl3_last_error(None)
