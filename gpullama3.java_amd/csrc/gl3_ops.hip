@@ -35,66 +35,93 @@ void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32
     });
 }
 
-uint64_t op_product_workspace(int64_t, int64_t, int32_t) { return 0; }
-
-// Which tile: the one with the least estimated time.  A stage of a BM x BN tile takes a CU 0.00164 (BM + BN) us for its operands' bytes + 0.0000101 BM BN us for its
-// MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 64 x 64 0.25), a tile 3 us and its results' bytes at 37 GB/s besides.  256 CUs take the
-// workgroups in rounds; two workgroups of a small tile share a CU.
-enum { OP_T256x256, OP_T128x256, OP_T256x128, OP_T128x128, OP_T64x128, OP_T64x64, OP_T_COUNT };
-static const struct { int bm, bn, share; } OP_TILES[OP_T_COUNT] = {{256, 256, 1}, {128, 256, 1}, {256, 128, 1}, {128, 128, 2}, {64, 128, 2}, {64, 64, 2}};
-static int op_ring_pick(int m, int n, int kp, int size, double* us_out) {
-    int best = 0;
-    double least = 1e300;
+// Which tile, and into how many parts its sum over k goes: the ones with the least estimated time.  A stage of a BM x BN tile takes a CU 0.00164 (BM + BN) us for
+// its operands' bytes + 0.0000101 BM BN us for its MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 64 x 64 0.25), a tile 3 us and its results'
+// bytes at 37 GB/s besides.  256 CUs take the workgroups in rounds; two workgroups of a small tile share a CU; the weights leave memory at 5.4 TB/s.  Tiles that are
+// too few for the CUs get their sums in parts of at least OP_PART_STAGES stages; a launch of its own adds them up, 2.5 us and what it reads (us, in parts / whole,
+// m tokens, n x k: 40, 4096 x 4096 10.9 / 12.3 (parts of 8 stages 12.5); 64, 4096 x 14336 17.7 / 36.1; 256 29.5 / 36.0; 64, 1024 x 4096 7.8 / 10.1; 64, 256 x 131000 24 / 254).
+enum { OP_T256x256, OP_T128x256, OP_T128x128, OP_T64x128, OP_T64x64, OP_T_COUNT };
+static const struct { int bm, bn, share; } OP_TILES[OP_T_COUNT] = {{256, 256, 1}, {128, 256, 1}, {128, 128, 2}, {64, 128, 2}, {64, 64, 2}};
+constexpr int OP_PART_STAGES = 4;
+struct OpRingPlan { int tile, parts; double us; };
+static OpRingPlan op_ring_plan(int m, int n, int kp, int size) {
+    OpRingPlan best{0, 1, 1e300};
+    const int stages = kp / 128;
+    const double memory = (double)n * kp / 5.4e6 + 4.0;
     for (int t = 0; t < OP_T_COUNT; ++t) {
         const int bm = OP_TILES[t].bm, bn = OP_TILES[t].bn, slots = 256 * OP_TILES[t].share;
-        const double one = kp / 128 * (0.00164 * (bm + bn) + 0.0000101 * bm * bn) + 3.0 + (double)bm * bn * size / 37e3;
+        const double stage = 0.00164 * (bm + bn) + 0.0000101 * bm * bn;
         const int64_t tiles = op_cdiv(m, bm) * op_cdiv(n, bn), rest = tiles % slots;
-        const double us = (double)(tiles / slots * OP_TILES[t].share + (rest == 0 ? 0 : rest <= 256 ? 1 : 2)) * one;
-        if (us < least) { least = us; best = t; }
+        const double rounds = (double)(tiles / slots * OP_TILES[t].share + (rest == 0 ? 0 : rest <= 256 ? 1 : 2));
+        const double whole = std::max(memory, rounds * (stages * stage + 3.0 + (double)bm * bn * size / 37e3));
+        if (whole < best.us) best = OpRingPlan{t, 1, whole};
+        const int parts = (int)std::min<int64_t>(std::min(256 / tiles, (int64_t)stages / OP_PART_STAGES), OP_MAX_PARTS);
+        if (parts < 2) continue;
+        const double split = std::max(memory, (double)op_cdiv(stages, parts) * stage + 3.0 + bm * bn * 4 / 37e3) + 2.5 + (double)m * n * 4 * parts / 2.5e6;
+        if (split < best.us) best = OpRingPlan{t, parts, split};
     }
-    *us_out = std::max(least, (double)n * kp / 5.4e6 + 4.0);          // the weights leave memory at 5.4 TB/s
     return best;
 }
 template <typename TY, int BM, int BN, int WM, int WN, int SA, int SW>
-static void op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p) {
+static void op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p, int parts) {
     const int mt = (int)op_cdiv(p.m, BM), nt = (int)op_cdiv(p.n, BN);
-    hipLaunchKernelGGL((op_ring_kernel<TY, BM, BN, WM, WN, SA, SW>), dim3((unsigned)op_cdiv((int64_t)mt * nt, 8) * 8), dim3(WM * WN * 64), 0, s, p, mt, nt);
+    hipLaunchKernelGGL((op_ring_kernel<TY, BM, BN, WM, WN, SA, SW>), dim3((unsigned)op_cdiv((int64_t)mt * nt, 8) * 8, (unsigned)parts), dim3(WM * WN * 64), 0, s, p, mt, nt);
 }
 template <typename TY>
-static void op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile) {
+static void op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile, int parts) {
     switch (tile) {
-        case OP_T256x256: op_ring_launch<TY, 256, 256, 4, 2, 2, 3>(s, p); break;
-        case OP_T128x256: op_ring_launch<TY, 128, 256, 2, 4, 2, 4>(s, p); break;
-        case OP_T256x128: op_ring_launch<TY, 256, 128, 4, 2, 3, 4>(s, p); break;
-        case OP_T128x128: op_ring_launch<TY, 128, 128, 2, 2, 2, 3>(s, p); break;
-        case OP_T64x128: op_ring_launch<TY, 64, 128, 2, 2, 2, 4>(s, p); break;
-        default: op_ring_launch<TY, 64, 64, 2, 2, 4, 5>(s, p);
+        case OP_T256x256: op_ring_launch<TY, 256, 256, 4, 2, 2, 3>(s, p, parts); break;
+        case OP_T128x256: op_ring_launch<TY, 128, 256, 2, 4, 2, 4>(s, p, parts); break;
+        case OP_T128x128: op_ring_launch<TY, 128, 128, 2, 2, 2, 3>(s, p, parts); break;
+        case OP_T64x128: op_ring_launch<TY, 64, 128, 2, 2, 2, 4>(s, p, parts); break;
+        default: op_ring_launch<TY, 64, 64, 2, 2, 4, 5>(s, p, parts);
     }
 }
 // Up to 32 tokens may be streamed: 6.6 TB/s of weights, 4.2 % more time a token (us, streamed / tiles; m tokens, n x k: 1, 4096 x 4096 6.5 / 10.3; 16 8.0 / 10.8;
-// 32 9.6 / 11.3; 16, 4096 x 14336 17.7 / 25.2; 4, 14336 x 4096 15.0 / 14.8; 8 16.5 / 14.8; 8, 32000 x 2048 16.2 / 14.0).  Eight wavefronts share the k of a strip
-// where there are few strips (4096 x 14336 12.6, four of them 14.5), four where they fill the chip (128256 x 4096 85.3, eight 86.5).
+// 24 9.1 / 11.6; 8, 4096 x 14336 14.6 / 15.9; 16 18.4 / 16.0; 4, 14336 x 4096 15.0 / 14.8; 8 16.5 / 14.8; 8, 32000 x 2048 16.2 / 14.0), and a strip alone takes
+// 26.6 KB a us, 3 % more time a token (16, 2560 x 9728 14.0 / 11.2; 16, 256 x 131000 117 / 21).  Eight wavefronts share the k of a strip where there are few strips
+// (4096 x 14336 12.6, four of them 14.5), four where they fill the chip (128256 x 4096 85.3, eight 86.5).
 constexpr int OP_FEW_STRIPS = 512;
-template <typename TY>
-static void op_product_piece(hipStream_t s, const OpProductArgs<TY>& p) {
-    double ring_us;
-    const int tile = op_ring_pick(p.m, p.n, p.kp, sizeof(TY), &ring_us);
-    if (p.m > 32 || 4.0 + (double)p.n * p.kp / 6.6e6 * (1.0 + 0.042 * p.m) > ring_us) { op_ring<TY>(s, p, tile); return; }
-    const unsigned strips = (unsigned)op_cdiv(p.n, 16);
-#define OP_STREAM(MT, KS, D) hipLaunchKernelGGL((op_stream_kernel<TY, MT, KS, D>), dim3(strips), dim3(64 * KS), 0, s, p)
-    if (strips <= OP_FEW_STRIPS) { if (p.m <= 16) OP_STREAM(1, 8, 4); else OP_STREAM(2, 8, 4); }
-    else { if (p.m <= 16) OP_STREAM(1, 4, 8); else OP_STREAM(2, 4, 8); }
-#undef OP_STREAM
+static bool op_streams(int m, int n, int kp, const OpRingPlan& ring) {
+    return m <= 32 && 4.0 + std::max((double)n * kp / 6.6e6 * (1.0 + 0.042 * m), kp / 1660.0 * (1.0 + 0.03 * m)) <= ring.us;
 }
-void op_product(hipStream_t s, const OpProduct& p, void*) {
-    constexpr int64_t PM = 1 << 16, PN = 1 << 18;          // a launch's rows and channels: its tiles have 32-bit numbers
+template <typename TY>
+static void op_product_piece(hipStream_t s, const OpProductArgs<TY>& p, void* workspace) {
+    const OpRingPlan ring = op_ring_plan(p.m, p.n, p.kp, sizeof(TY));
+    if (op_streams(p.m, p.n, p.kp, ring)) {
+        const unsigned strips = (unsigned)op_cdiv(p.n, 16);
+#define OP_STREAM(MT, KS, D) hipLaunchKernelGGL((op_stream_kernel<TY, MT, KS, D>), dim3(strips), dim3(64 * KS), 0, s, p)
+        if (strips <= OP_FEW_STRIPS) { if (p.m <= 16) OP_STREAM(1, 8, 4); else OP_STREAM(2, 8, 4); }
+        else { if (p.m <= 16) OP_STREAM(1, 4, 8); else OP_STREAM(2, 4, 8); }
+#undef OP_STREAM
+    } else if (ring.parts == 1) op_ring<TY>(s, p, ring.tile, 1);
+    else {
+        op_ring<int>(s, OpProductArgs<int>{p.a, p.lda, nullptr, p.w, p.ldw, nullptr, nullptr, p.m, p.n, p.kp, (int*)workspace, p.n}, ring.tile, ring.parts);
+        hipLaunchKernelGGL((op_parts_kernel<TY>), dim3((unsigned)op_cdiv(p.n, 256), (unsigned)p.m), dim3(256), 0, s, (const int*)workspace, ring.parts, p);
+    }
+}
+constexpr int64_t OP_PM = 1 << 16, OP_PN = 1 << 18;          // a launch's rows and channels: its tiles have 32-bit numbers
+void op_product(hipStream_t s, const OpProduct& p, void* workspace) {
     op_with_type(p.y_type, [&](auto t) {
         typedef decltype(t) TY;
-        for (int64_t n = 0; n < p.n; n += PN)
-            for (int64_t m = 0; m < p.m; m += PM)
-                op_product_piece(s, OpProductArgs<TY>{p.a + m * p.lda, p.lda, p.a_scale + m, p.w + n * p.ldw, p.ldw, p.w_scale + n, p.bias ? p.bias + n : nullptr, (int)std::min(PM, p.m - m),
-                                                      (int)std::min(PN, p.n - n), (int)op_code_ld(p.k), (TY*)p.y + m * p.ldy + n, p.ldy});
+        for (int64_t n = 0; n < p.n; n += OP_PN)
+            for (int64_t m = 0; m < p.m; m += OP_PM)
+                op_product_piece(s, OpProductArgs<TY>{p.a + m * p.lda, p.lda, p.a_scale + m, p.w + n * p.ldw, p.ldw, p.w_scale + n, p.bias ? p.bias + n : nullptr, (int)std::min(OP_PM, p.m - m),
+                                                      (int)std::min(OP_PN, p.n - n), (int)op_code_ld(p.k), (TY*)p.y + m * p.ldy + n, p.ldy}, workspace);
     });
+}
+// the parts of the piece that needs most (whatever the results' type); pieces run one after the other
+uint64_t op_product_workspace(int64_t m, int64_t n, int32_t k) {
+    const int kp = (int)op_code_ld(k);
+    uint64_t most = 0;
+    const int64_t ms[2] = {std::min(m, OP_PM), m > OP_PM ? m % OP_PM : 0}, ns[2] = {std::min(n, OP_PN), n > OP_PN ? n % OP_PN : 0};
+    for (int64_t pm : ms)
+        for (int64_t pn : ns)
+            for (int size = 2; pm && pn && size <= 4; size += 2) {
+                const OpRingPlan ring = op_ring_plan((int)pm, (int)pn, kp, size);
+                if (ring.parts > 1 && !op_streams((int)pm, (int)pn, kp, ring)) most = std::max<uint64_t>(most, (uint64_t)pm * pn * ring.parts * 4);
+            }
+    return most;
 }
 
 constexpr int OP_TOKEN_STRIPS = 2048;

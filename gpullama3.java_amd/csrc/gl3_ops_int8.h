@@ -269,8 +269,10 @@ __device__ __forceinline__ void op_dma16(const void* src, void* lds) {
 template <int I, int N, typename F> __device__ __forceinline__ void op_static_for(F f) { if constexpr (I < N) { f(std::integral_constant<int, I>{}); op_static_for<I + 1, N>(f); } }
 template <int N> __device__ __forceinline__ void op_wait_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory"); }
 
+// TY = int: part blockIdx.y of gridDim.y of the sum over k, y[part][m][ldy] (op_parts_kernel adds them up).
 template <typename TY, int BM, int BN, int WM, int WN, int SA, int SW>
 static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProductArgs<TY> p, int mt, int nt) {
+    constexpr bool PART = std::is_same<TY, int>::value;
     constexpr int NW = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
     constexpr int PA = BM / 8, PW = BN / 8, NPA = (PA + NW - 1) / NW, NPW = (PW + NW - 1) / NW, NP = NPA + NPW;          // 1 KB pieces (8 rows) of a stage, per wavefront
     constexpr int SZA = BM * 128, SZW = BN * 128, OW = SA * SZA;
@@ -280,8 +282,10 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wm = wave / WN, wn = wave % WN;
     const int total = mt * nt, per_xcd = (total + 7) >> 3, J = (blockIdx.x & 7) * per_xcd + (blockIdx.x >> 3);
     if (J >= total) return;
-    const int m0 = (J % mt) * BM, n0 = (J / mt) * BN, n_it = p.kp / 128;
-    const int8_t *ab = p.a + m0 * p.lda, *wb = p.w + n0 * p.ldw;
+    const int m0 = (J % mt) * BM, n0 = (J / mt) * BN, stages = p.kp / 128;
+    const int it0 = PART ? stages * (int)blockIdx.y / (int)gridDim.y : 0, n_it = PART ? stages * ((int)blockIdx.y + 1) / (int)gridDim.y - it0 : stages;
+    const int8_t *ab = p.a + m0 * p.lda + it0 * 128, *wb = p.w + n0 * p.ldw + it0 * 128;
+    if constexpr (PART) p.y += (int64_t)blockIdx.y * p.m * p.ldy;
     // this wavefront's pieces (rows past the end repeat the last one: their results are not stored; wavefronts without a piece of their own load one again)
     uint32_t offa[NPA], offw[NPW];
     int pa[NPA], pw[NPW];
@@ -299,7 +303,7 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
     }
     // scales of the tile's rows and columns, one a thread: needed at the end, in LDS
     const int my_m = min(m0 + (tid < BM ? tid : 0), p.m - 1), my_n = min(n0 + (tid < BN ? tid : 0), p.n - 1);
-    const float my_as = p.as[my_m], my_ws = p.ws[my_n], my_b = p.bias ? p.bias[my_n] : 0.f;
+    const float my_as = PART ? 0.f : p.as[my_m], my_ws = PART ? 0.f : p.ws[my_n], my_b = !PART && p.bias ? p.bias[my_n] : 0.f;
     constexpr int WH = (NPW + 1) / 2;
     auto issue_a = [&](int it, int slot) {
         const int8_t* a = ab + (int64_t)it * 128;
@@ -397,9 +401,11 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
     // Lane holds channel lane % 32 and tokens 8 (r / 4) + 4 (lane / 32) + r % 4 of every 32 x 32 tile.  A store's row comes from the scalar unit, the lane's
     // part is one 32-bit offset.  (Behind the last barrier nobody reads the rings and no load is on its way.)
     float *las = reinterpret_cast<float*>(smem), *lws = las + BM, *lb = lws + BN;
-    if (tid < BM) las[tid] = my_as;
-    if (tid < BN) { lws[tid] = my_ws; lb[tid] = my_b; }
-    __syncthreads();
+    if constexpr (!PART) {
+        if (tid < BM) las[tid] = my_as;
+        if (tid < BN) { lws[tid] = my_ws; lb[tid] = my_b; }
+        __syncthreads();
+    }
     const int mb = m0 + wm * (BM / WM), nb = n0 + wn * (BN / WN);
     const bool whole = m0 + BM <= p.m && n0 + BN <= p.n, biased = p.bias != nullptr;
     const uint32_t lo = ((uint32_t)(4 * kh) * (uint32_t)p.ldy + r32) * (uint32_t)sizeof(TY);
@@ -407,7 +413,7 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
         constexpr bool ALL = decltype(all)::value;
         float w_[TN], b_[TN];
 #pragma unroll
-        for (int j = 0; j < TN; ++j) { const int c = wn * (BN / WN) + j * 32 + r32; w_[j] = lws[c]; b_[j] = lb[c]; }
+        for (int j = 0; j < TN; ++j) { const int c = wn * (BN / WN) + j * 32 + r32; w_[j] = PART ? 0.f : lws[c]; b_[j] = PART ? 0.f : lb[c]; }
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
@@ -419,11 +425,32 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
                     uint8_t* y = reinterpret_cast<uint8_t*>(p.y + row * p.ldy + nb);
 #pragma unroll
                     for (int j = 0; j < TN; ++j) {          // (a row's columns one behind the other: with the rows inside, 13.4 us a float32 tile of 256 x 256 instead of 5)
-                        const float x = op_result(acc[i][j][4 * g + r], s4[r], w_[j]);
-                        if (ALL || (row + 4 * kh < p.m && nb + j * 32 + r32 < p.n)) op_store_past(reinterpret_cast<TY*>(y + j * 32 * sizeof(TY) + lo), op_cast<TY>(biased ? x + b_[j] : x));
+                        const bool in = ALL || (row + 4 * kh < p.m && nb + j * 32 + r32 < p.n);
+                        TY* at = reinterpret_cast<TY*>(y + j * 32 * sizeof(TY) + lo);
+                        if constexpr (PART) { if (in) *at = acc[i][j][4 * g + r]; }
+                        else {
+                            const float x = op_result(acc[i][j][4 * g + r], s4[r], w_[j]);
+                            if (in) op_store_past(at, op_cast<TY>(biased ? x + b_[j] : x));
+                        }
                     }
                 }
             }
     };
     if (whole) store(std::true_type{}); else store(std::false_type{});
+}
+
+// The parts of a product's sums, added up: grid (n / 256, m), a result a thread.
+constexpr int OP_MAX_PARTS = 16;
+template <typename TY>
+static __global__ __launch_bounds__(256) void op_parts_kernel(const int* __restrict__ parts, int count, OpProductArgs<TY> p) {
+    const int col = (int)blockIdx.x * 256 + threadIdx.x, row = blockIdx.y;
+    if (col >= p.n) return;
+    int v[OP_MAX_PARTS];
+#pragma unroll
+    for (int i = 0; i < OP_MAX_PARTS; ++i) v[i] = i < count ? parts[((int64_t)i * p.m + row) * p.n + col] : 0;
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < OP_MAX_PARTS; ++i) sum += v[i];
+    const float x = op_result(sum, p.as[row], p.ws[col]);
+    p.y[(int64_t)row * p.ldy + col] = op_cast<TY>(p.bias ? x + p.bias[col] : x);
 }

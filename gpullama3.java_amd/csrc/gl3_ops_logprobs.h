@@ -68,7 +68,6 @@ __device__ __forceinline__ float op_uniform(float v) { return __uint_as_float(__
 constexpr int OP_LP_THREADS = 256, OP_LP_WAVES = OP_LP_THREADS / 64;
 
 struct OpSums { float m, s, t; };          // m = -inf: no logit above -inf so far (s is 0, or NaN)
-__device__ __forceinline__ float op_scale(float from, float to) { return from == -INFINITY ? 1.f : __expf(from - to); }
 __device__ __forceinline__ OpSums op_rescale(OpSums a, float m) {          // to a larger maximum
     if (a.m == m || a.m == -INFINITY) { a.m = m; return a; }
     const float d = a.m - m, e = __expf(d);
@@ -106,7 +105,7 @@ struct OpTop {
         lo = fmaxf(lo, fmaxf(logit(__builtin_amdgcn_readlane(ord, top - 1)), logit(__builtin_amdgcn_readfirstlane(least))));
     }
     // 64 of the collected candidates, or what is left of them, into the list
-    __device__ __forceinline__ void merge(uint64_t* buf, int top, int lane) {
+    __device__ __forceinline__ void merge(uint64_t* buf, int lane) {
         const int first = max(0, n - 64);
         const uint64_t c = first + lane < n ? buf[first + lane] : 0;
         n = first;
@@ -247,7 +246,7 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 5) void op_logprobs_kernel(co
                     }
                 i0 = next;
                 if (best.n >= 64) {
-                    do best.merge(buf, o.top, lane); while (best.n >= 64);
+                    do best.merge(buf, lane); while (best.n >= 64);
                     best.raise(o.top, lane);
                 }
             }
@@ -292,7 +291,7 @@ static __global__ __launch_bounds__(OP_LP_THREADS, 5) void op_logprobs_kernel(co
         }
     }
     if constexpr (TOP) {
-        while (best.n >= 64) best.merge(buf, o.top, lane);
+        while (best.n >= 64) best.merge(buf, lane);
         if (best.any_key) buf[64 + lane] = best.key;
         if (lane == 0) got_s[wave] = best.n | (best.any_key ? 256 : 0);
     }
@@ -381,7 +380,7 @@ static __global__ __launch_bounds__(64 * OP_LP_JOIN_WAVES) void op_logprobs_join
         __syncthreads();
         if (wave == 0) {
             best.n = count;
-            while (best.n) best.merge(buf, top, lane);
+            while (best.n) best.merge(buf, lane);
         }
     }
     if (wave) return;

@@ -130,12 +130,15 @@ def test_errors_belong_to_the_thread(hip):
     assert all((b"top" in next(iter(v))) == bool(i % 2) for i, v in seen.items())
 
 
-@pytest.mark.parametrize("i", range(9))
-def test_strides_beyond_the_documented_ones(hip, i):
+@pytest.mark.parametrize("i", range(12))
+def test_strides_and_workspaces_that_do_not_do(hip, i):
     name, make, kw = [("gl3_int8_matmul", matmul, dict(ldw=(1 << 23) + 16)), ("gl3_int8_matmul", matmul, dict(lda=(1 << 23) + 16)), ("gl3_int8_matmul", matmul, dict(ldy=(1 << 26) + 1)),
                       ("gl3_int8_linear", linear, dict(ldw=(1 << 23) + 16)), ("gl3_int8_linear", linear, dict(ldy=(1 << 26) + 1)), ("gl3_int8_linear", linear, dict(ldx=1 << 62)),
                       ("gl3_token_logprobs", logprobs, dict(vocab=(1 << 30) + 1, ld=(1 << 30) + 1)), ("gl3_token_logprobs", logprobs, dict(ld=1 << 62)),
-                      ("gl3_token_logprobs", logprobs, dict(vocab=128256, ld=128256, bytes=100))][i]
+                      ("gl3_token_logprobs", logprobs, dict(vocab=128256, ld=128256, bytes=100)),
+                      ("gl3_int8_matmul", matmul, dict(m=40, n=300, k=9000, lda=9088, ldw=9088, ldy=300, workspace=None, bytes=0)),
+                      ("gl3_int8_matmul", matmul, dict(m=40, n=300, k=9000, lda=9088, ldw=9088, ldy=300, bytes=40 * 300 * 4)),
+                      ("gl3_int8_linear", linear, dict(m=40, n=300, k=9000, ldx=9000, ldw=9088, ldy=300, bytes=40 * 9088 + 160))][i]
     assert getattr(hip.lib(), name)(*make(**kw)) == hip.E_ARG, (name, kw)
 
 

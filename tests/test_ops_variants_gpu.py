@@ -1,0 +1,197 @@
+"""Operators on device memory where their sizes change the kernel: every tile and strip with few and many stages, rows of every length, launches in
+pieces, offsets that pass 32 bits, another stream's and the default stream's calls."""
+from importlib import import_module
+
+import numpy as np
+import pytest
+import torch
+
+import __graft_entry__ as ge
+from test_ops_gpu import DEV, NAMES, check_product, check_rows, codes_of, int8_rows, odd_rows, rng, targets_of
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops(pkg):
+    return import_module(ge.PKG_NAME + ".ops")
+
+
+@pytest.fixture(scope="module")
+def hip(pkg):
+    return import_module(ge.PKG_NAME + ".hip")
+
+
+# ---- products: m x n chooses the kernel (a few tokens: strips; else the tile), k the number of stages of 128 columns, fewer and more than the rings hold ----
+@pytest.mark.parametrize("stages", [1, 2, 3, 4, 5, 7])
+@pytest.mark.parametrize("m,n", [(3, 700), (5, 8203), (17, 700), (17, 33000), (100, 700), (33, 16385), (70, 16390), (33, 33000), (8385, 842), (390, 16390)])
+def test_stages(ops, m, n, stages):
+    k = stages * 128 - (stages * 37 + m) % 128
+    a, w = int8_rows(ops, m, k, m), int8_rows(ops, n, k, n + 1)
+    bias = torch.from_numpy(rng(3).standard_normal(n).astype(np.float32)).to(DEV)
+    check_product(ops.int8_matmul(a, w), a, w)
+    check_product(ops.int8_matmul(a, w, bias, torch.bfloat16), a, w, bias)
+
+
+@pytest.mark.parametrize("m,n,k", [(40, 300, 9000), (33, 64, 1024), (64, 1024, 4096), (1, 20, 131071), (17, 64, 8192), (24, 257, 30000), (65, 1000, 14336), (130, 500, 5000), (257, 513, 4100), (300, 1500, 1025)])
+def test_sums_in_parts(ops, m, n, k):
+    """Few tiles and a long k: every part's sums meet, beside each of the epilogue's forms."""
+    a, w = int8_rows(ops, m, k, m, extra=16), int8_rows(ops, n, k, n + 1)
+    bias = torch.from_numpy(rng(3).standard_normal(n).astype(np.float32)).to(DEV)
+    for t in NAMES.values():
+        wide = torch.full((m + 1, n + 3), 3.0, dtype=t, device=DEV)
+        check_product(ops.int8_matmul(a, w, bias, t, out=wide[:m, 1:n + 1]), a, w, bias)
+        assert (wide[m] == 3).all() and (wide[:, 0] == 3).all() and (wide[:, n + 1:] == 3).all()
+    x = torch.from_numpy(odd_rows(m, k, 5)).to(DEV)
+    y = ops.int8_linear(x, w)
+    assert torch.equal(y, ops.int8_matmul(ops.quantize_rows(x), w))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        z = ops.int8_linear(x, w)
+    for i in range(3):
+        x.copy_(torch.from_numpy(odd_rows(m, k, 6 + i)))
+        g.replay()
+        y = ops.int8_linear(x, w)
+        torch.cuda.synchronize()
+        assert torch.equal(z, y)
+
+
+@pytest.mark.parametrize("n,k", [(9001, 130), (9001, 8192), (9001, 8193), (20, 16384), (20, 16385), (32768, 300), (32769, 300), (5, 1)])
+def test_one_token(ops, n, k):
+    w = int8_rows(ops, n, k, 4)
+    for t in NAMES.values():
+        x = torch.from_numpy(odd_rows(1, k, k)).to(t).to(DEV)
+        x = torch.where(torch.isfinite(x), x, torch.ones_like(x))
+        a = ops.quantize_rows(x)
+        y = ops.int8_linear(x, w, dtype=torch.float32)
+        assert torch.equal(y, ops.int8_matmul(a, w))
+        check_product(y, a, w)
+
+
+@pytest.mark.parametrize("rows,cols", [(3000, 700), (3000, 2048), (3000, 2049), (70, 5000), (70, 8192), (70, 8193), (64, 8192), (3, 9000), (2, 32768), (2, 32769), (3, 512), (3, 513), (5, 2049)])
+def test_codes_of_rows_of_every_length(ops, rows, cols):
+    for dtype in NAMES:
+        x = torch.from_numpy(odd_rows(rows, cols + 1, rows + cols))
+        if dtype == "f16":
+            x.clamp_(-60000, 60000)
+        x = x.to(NAMES[dtype])[:, 1:]
+        got = ops.quantize_rows(x.to(DEV))
+        q, s = codes_of(x.float().numpy())
+        assert np.array_equal(got.scale.cpu().numpy(), s) and np.array_equal(got.codes.cpu().numpy()[:, :cols], q) and not got.codes[:, cols:].any()
+
+
+@pytest.mark.parametrize("m,n,k", [(65536 + 130, 40, 70), (1, 262144 + 77, 130), (3, 262144 + 77, 130), (40, 262144 + 77, 130)])
+def test_products_in_pieces(ops, m, n, k):
+    a, w = int8_rows(ops, m, k, 1), int8_rows(ops, n, k, 2)
+    bias = torch.from_numpy(rng(3).standard_normal(n).astype(np.float32)).to(DEV)
+    check_product(ops.int8_matmul(a, w, bias), a, w, bias)
+
+
+def test_more_rows_of_logits_than_a_launch_takes(ops):
+    rows, vocab = 65535 + 1200, 9
+    x = torch.from_numpy(rng(1).standard_normal((rows, vocab)).astype(np.float32)).to(DEV)
+    t = targets_of(rows, vocab, 2, low=-1)
+    got = ops.token_logprobs(x, t, 3)
+    for lo, hi in ((0, 300), (65400, 65700), (rows - 300, rows)):
+        check_rows(type(got)(*(v[lo:hi] for v in got)), x[lo:hi], t[lo:hi], 3)
+    lp = torch.log_softmax(x.double(), 1)
+    assert torch.allclose(got.top_logprobs[:, 0].double(), lp.max(1).values, rtol=0, atol=1e-5)
+
+
+# ---- offsets that pass 32 bits: the last rows are what they are on their own ----
+def test_results_past_32_bits(ops):
+    m, n = 16800, 128256          # 2.15 G results
+    a = ops.Int8Rows(torch.randint(-127, 128, (m, 128), dtype=torch.int8, device=DEV), torch.rand(m, device=DEV), 128)
+    w = ops.Int8Rows(torch.randint(-127, 128, (n, 128), dtype=torch.int8, device=DEV), torch.rand(n, device=DEV), 128)
+    y = ops.int8_matmul(a, w, None, torch.bfloat16)
+    for lo in (0, 8000, m - 70):
+        part = ops.Int8Rows(a.codes[lo:lo + 70], a.scale[lo:lo + 70], 128)
+        assert torch.equal(y[lo:lo + 70], ops.int8_matmul(part, w, None, torch.bfloat16))
+    part = ops.Int8Rows(a.codes[m - 5:], a.scale[m - 5:], 128)
+    check_product(y[m - 5:], part, w)
+    # rows of logits, and rows to be quantised, that start behind 2^31 elements
+    t = torch.full((m,), 77, dtype=torch.int32, device=DEV)
+    got = ops.token_logprobs(y, t, 2)
+    for lo in (0, m - 3):
+        check_rows(type(got)(*(v[lo:lo + 3] for v in got)), y[lo:lo + 3], t[lo:lo + 3], 2)
+    q = ops.quantize_rows(y)
+    last = ops.quantize_rows(y[m - 40:])
+    assert torch.equal(q.codes[m - 40:], last.codes) and torch.equal(q.scale[m - 40:], last.scale)
+    c, s = codes_of(y[m - 2:].float().cpu().numpy())
+    assert np.array_equal(q.codes[m - 2:].cpu().numpy()[:, :n], c) and np.array_equal(q.scale[m - 2:].cpu().numpy(), s)
+
+
+@pytest.mark.parametrize("m", [1, 20, 70, 300])
+def test_weights_past_32_bits(ops, m):
+    n, k = 262000, 8200          # 2.18 GB of codes
+    w = ops.Int8Rows(torch.randint(-127, 128, (n, 8320), dtype=torch.int8, device=DEV), torch.rand(n, device=DEV), k)
+    w.codes[:, k:] = 0
+    x = torch.randn(m, k, device=DEV)
+    y = ops.int8_linear(x, w)
+    for lo in (0, n - 300):
+        part = ops.Int8Rows(w.codes[lo:lo + 300], w.scale[lo:lo + 300].clone(), k)
+        assert torch.equal(y[:, lo:lo + 300], ops.int8_linear(x, part))
+    check_product(y[:, n - 300:], ops.quantize_rows(x), ops.Int8Rows(w.codes[n - 300:], w.scale[n - 300:].clone(), k))
+
+
+# ---- calls ----
+def test_the_default_stream(ops, hip):
+    """Stream NULL from C, with a workspace of the caller."""
+    import ctypes as C
+    L = hip.lib()
+    m, n, k, vocab = 7, 300, 200, 300
+    x = torch.from_numpy(odd_rows(m, k, 1)).to(DEV)
+    w = int8_rows(ops, n, k, 2)
+    nbytes, need = C.c_uint64(), C.c_uint64()
+    assert L.gl3_int8_workspace(m, n, k, None, C.byref(nbytes)) == 0 and L.gl3_logprobs_workspace(m, vocab, 5, C.byref(need)) == 0
+    ws = torch.empty(max(nbytes.value, need.value, 16), dtype=torch.uint8, device=DEV)
+    y = torch.empty(m, n, device=DEV)
+    t = torch.zeros(m, dtype=torch.int32, device=DEV)
+    lp, rank, ids, values = torch.empty(m, device=DEV), torch.empty(m, dtype=torch.int32, device=DEV), torch.empty(m, 5, dtype=torch.int32, device=DEV), torch.empty(m, 5, device=DEV)
+    torch.cuda.synchronize()
+    assert L.gl3_int8_linear(0, None, x.data_ptr(), 0, k, w.codes.data_ptr(), w.ld, w.scale.data_ptr(), None, m, n, k, y.data_ptr(), 0, n, ws.data_ptr(), nbytes.value) == 0
+    assert L.gl3_token_logprobs(0, None, y.data_ptr(), 0, m, vocab, n, t.data_ptr(), 5, lp.data_ptr(), rank.data_ptr(), None, ids.data_ptr(), values.data_ptr(), ws.data_ptr(), need.value) == 0
+    torch.cuda.synchronize()
+    check_product(y, ops.quantize_rows(x), w)
+    want = ops.token_logprobs(y, t, 5)
+    assert torch.equal(lp, want.logprob) and torch.equal(rank, want.rank) and torch.equal(ids, want.top_ids) and torch.equal(values, want.top_logprobs)
+
+
+def test_rows_that_overlap_are_refused(ops, hip):
+    """A broadcast row and sliding windows have a stride below a row's length."""
+    w = int8_rows(ops, 10, 100, 1)
+    x = torch.randn(1, 100, device=DEV)
+    for bad in (x.expand(4, 100), torch.randn(400, device=DEV).as_strided((4, 100), (50, 1))):
+        for call in (lambda: ops.quantize_rows(bad), lambda: ops.int8_linear(bad, w), lambda: ops.token_logprobs(bad)):
+            with pytest.raises(hip.Gl3Error):
+                call()
+    with pytest.raises(hip.Gl3Error):
+        ops.int8_linear(torch.randn(4, 100, device=DEV), w, dtype=torch.float32, out=torch.zeros(1, 10, device=DEV).expand(4, 10))
+    assert ops.int8_linear(x, w).shape == (1, 10)
+
+
+def test_two_graphs_with_workspaces_of_their_own(ops):
+    """Replayed at the same time on two streams, each as it is alone."""
+    w = int8_rows(ops, 3001, 768, 1)
+    graphs, outs, xs = [], [], []
+    for i in range(2):
+        x = torch.from_numpy(odd_rows(60, 768, i)).to(DEV)
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            ops.token_logprobs(ops.int8_linear(x, w), None, 5)
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            outs.append(ops.token_logprobs(ops.int8_linear(x, w), None, 5))
+        graphs.append(g); xs.append(x)
+    want = [ops.token_logprobs(ops.int8_linear(x, w), None, 5) for x in xs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        for g, s in zip(graphs, streams):
+            with torch.cuda.stream(s):
+                g.replay()
+        torch.cuda.synchronize()
+        for got, ref in zip(outs, want):
+            assert torch.equal(got.top_ids, ref.top_ids) and torch.equal(got.top_logprobs, ref.top_logprobs) and torch.equal(got.entropy, ref.entropy)
