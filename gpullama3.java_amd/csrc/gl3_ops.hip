@@ -36,12 +36,12 @@ void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32
 }
 
 // Which tile, and into how many parts its sum over k goes: the ones with the least estimated time.  A stage of a BM x BN tile takes a CU 0.00164 (BM + BN) us for
-// its operands' bytes + 0.0000101 BM BN us for its MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 64 x 64 0.25), a tile 3 us and its results'
+// its operands' bytes + 0.0000101 BM BN us for its MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 32 x 128 0.30, 64 x 64 0.25), a tile 3 us and its results'
 // bytes at 37 GB/s besides.  256 CUs take the workgroups in rounds; two workgroups of a small tile share a CU; the weights leave memory at 5.4 TB/s.  Tiles that are
 // too few for the CUs get their sums in parts of at least OP_PART_STAGES stages; a launch of its own adds them up, 2.5 us and what it reads (us, in parts / whole,
 // m tokens, n x k: 40, 4096 x 4096 10.9 / 12.3 (parts of 8 stages 12.5); 64, 4096 x 14336 17.7 / 36.1; 256 29.5 / 36.0; 64, 1024 x 4096 7.8 / 10.1; 64, 256 x 131000 24 / 254).
-enum { OP_T256x256, OP_T128x256, OP_T128x128, OP_T64x128, OP_T64x64, OP_T_COUNT };
-static const struct { int bm, bn, share; } OP_TILES[OP_T_COUNT] = {{256, 256, 1}, {128, 256, 1}, {128, 128, 2}, {64, 128, 2}, {64, 64, 2}};
+enum { OP_T256x256, OP_T128x256, OP_T128x128, OP_T64x128, OP_T64x64, OP_T32x128, OP_T_COUNT };
+static const struct { int bm, bn, share; } OP_TILES[OP_T_COUNT] = {{256, 256, 1}, {128, 256, 1}, {128, 128, 2}, {64, 128, 2}, {64, 64, 2}, {32, 128, 2}};
 constexpr int OP_PART_STAGES = 4;
 struct OpRingPlan { int tile, parts; double us; };
 static OpRingPlan op_ring_plan(int m, int n, int kp, int size) {
@@ -53,11 +53,11 @@ static OpRingPlan op_ring_plan(int m, int n, int kp, int size) {
         const double stage = 0.00164 * (bm + bn) + 0.0000101 * bm * bn;
         const int64_t tiles = op_cdiv(m, bm) * op_cdiv(n, bn), rest = tiles % slots;
         const double rounds = (double)(tiles / slots * OP_TILES[t].share + (rest == 0 ? 0 : rest <= 256 ? 1 : 2));
-        const double whole = std::max(memory, rounds * (stages * stage + 3.0 + (double)bm * bn * size / 37e3));
+        const double busy = rounds * (stages * stage + 3.0 + (double)bm * bn * size / 37e3), whole = std::max(memory, busy) + 1e-3 * busy;          // (of several that memory holds up, the least busy)
         if (whole < best.us) best = OpRingPlan{t, 1, whole};
         const int parts = (int)std::min<int64_t>(std::min(256 / tiles, (int64_t)stages / OP_PART_STAGES), OP_MAX_PARTS);
-        if (parts < 2) continue;
-        const double split = std::max(memory, (double)op_cdiv(stages, parts) * stage + 3.0 + bm * bn * 4 / 37e3) + 2.5 + (double)m * n * 4 * parts / 2.5e6;
+        if (parts < 2 || bn > 128) continue;          // (parts of the larger tiles: 45.2 us, whole 46.1, at 142 tokens, 11037 x 9472)
+        const double part = (double)op_cdiv(stages, parts) * stage + 3.0 + bm * bn * 4 / 37e3, split = std::max(memory, part) + 1e-3 * part + 2.5 + (double)m * n * 4 * parts / 2.5e6;
         if (split < best.us) best = OpRingPlan{t, parts, split};
     }
     return best;
@@ -69,12 +69,15 @@ static void op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p, int parts)
 }
 template <typename TY>
 static void op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile, int parts) {
+    if constexpr (!std::is_same<TY, int>::value) {          // (tiles that are never in parts)
+        if (tile == OP_T256x256) return op_ring_launch<TY, 256, 256, 4, 2, 2, 3>(s, p, parts);
+        if (tile == OP_T128x256) return op_ring_launch<TY, 128, 256, 2, 4, 2, 4>(s, p, parts);
+    }
     switch (tile) {
-        case OP_T256x256: op_ring_launch<TY, 256, 256, 4, 2, 2, 3>(s, p, parts); break;
-        case OP_T128x256: op_ring_launch<TY, 128, 256, 2, 4, 2, 4>(s, p, parts); break;
         case OP_T128x128: op_ring_launch<TY, 128, 128, 2, 2, 2, 3>(s, p, parts); break;
         case OP_T64x128: op_ring_launch<TY, 64, 128, 2, 2, 2, 4>(s, p, parts); break;
-        default: op_ring_launch<TY, 64, 64, 2, 2, 4, 5>(s, p, parts);
+        case OP_T64x64: op_ring_launch<TY, 64, 64, 2, 2, 4, 5>(s, p, parts); break;
+        default: op_ring_launch<TY, 32, 128, 1, 4, 3, 4>(s, p, parts);          // (rings of 2 and 4: 81 us instead of 77 at 32 tokens, 151936 x 2560)
     }
 }
 // Up to 32 tokens may be streamed: 6.6 TB/s of weights, 4.2 % more time a token (us, streamed / tiles; m tokens, n x k: 1, 4096 x 4096 6.5 / 10.3; 16 8.0 / 10.8;

@@ -113,10 +113,13 @@ def quantize_rows(x: torch.Tensor) -> Int8Rows:
     if not 0 < cols <= MAX_K:
         raise _bad("x must have 1 .. %d columns" % MAX_K)
     device = x.device
-    codes = torch.empty(rows, -(-cols // CODE_BLOCK) * CODE_BLOCK, dtype=torch.int8, device=device)
+    ld_codes = -(-cols // CODE_BLOCK) * CODE_BLOCK
+    codes = torch.empty(rows, ld_codes, dtype=torch.int8, device=device)
     scale = torch.empty(rows, dtype=torch.float32, device=device)
-    _call(hip.lib().gl3_quantize_rows, device, x.data_ptr(), _TYPES[x.dtype], rows, cols, ld, codes.data_ptr(), codes.shape[1], scale.data_ptr())
-    return Int8Rows(codes, scale, cols)
+    _call(hip.lib().gl3_quantize_rows, device, x.data_ptr(), _TYPES[x.dtype], rows, cols, ld, codes.data_ptr(), ld_codes, scale.data_ptr())
+    r = Int8Rows.__new__(Int8Rows)          # (made here: nothing to check)
+    r.codes, r.scale, r.cols, r.rows, r.ld, r.device = codes, scale, cols, rows, ld_codes, device
+    return r
 
 
 def _result(w, bias, m, k, dtype, out, device):

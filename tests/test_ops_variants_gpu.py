@@ -24,7 +24,7 @@ def hip(pkg):
 
 # ---- products: m x n chooses the kernel (a few tokens: strips; else the tile), k the number of stages of 128 columns, fewer and more than the rings hold ----
 @pytest.mark.parametrize("stages", [1, 2, 3, 4, 5, 7])
-@pytest.mark.parametrize("m,n", [(3, 700), (5, 8203), (17, 700), (17, 33000), (100, 700), (33, 16385), (70, 16390), (33, 33000), (8385, 842), (390, 16390)])
+@pytest.mark.parametrize("m,n", [(3, 700), (5, 8203), (17, 700), (17, 33000), (100, 700), (33, 16385), (70, 16390), (33, 33000), (31, 20001), (8385, 842), (390, 16390)])
 def test_stages(ops, m, n, stages):
     k = stages * 128 - (stages * 37 + m) % 128
     a, w = int8_rows(ops, m, k, m), int8_rows(ops, n, k, n + 1)
@@ -33,7 +33,8 @@ def test_stages(ops, m, n, stages):
     check_product(ops.int8_matmul(a, w, bias, torch.bfloat16), a, w, bias)
 
 
-@pytest.mark.parametrize("m,n,k", [(40, 300, 9000), (33, 64, 1024), (64, 1024, 4096), (1, 20, 131071), (17, 64, 8192), (24, 257, 30000), (65, 1000, 14336), (130, 500, 5000), (257, 513, 4100), (300, 1500, 1025)])
+@pytest.mark.parametrize("m,n,k", [(40, 300, 9000), (33, 64, 1024), (64, 1024, 4096), (1, 20, 131071), (17, 64, 8192), (24, 257, 30000), (65, 1000, 14336), (130, 500, 5000), (257, 513, 4100), (300, 1500, 1025), (35, 1189, 6600), (142, 1000, 30000),
+                                   (512, 1024, 10000), (2758, 66, 4352)])
 def test_sums_in_parts(ops, m, n, k):
     """Few tiles and a long k: every part's sums meet, beside each of the epilogue's forms."""
     a, w = int8_rows(ops, m, k, m, extra=16), int8_rows(ops, n, k, n + 1)
