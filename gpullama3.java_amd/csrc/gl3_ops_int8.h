@@ -79,7 +79,7 @@ template <typename T, int NV, int NT> struct OpRowPart {
     }
 };
 // W wavefronts a row, 4 / W rows a workgroup (one where W > 4); the row stays in registers between its largest value and its codes: one read, one write.
-// kp <= OP_ROW_E x 64 W.  (Two passes over memory, one element a thread and step: 8192 columns of one row 11.5 us in front of a product, 2041 x 4096 bfloat16 12.8.)
+// kp <= OP_ROW_E x 64 W.  2041 x 4096 bfloat16 9.4 us, a few rows 4 .. 5: little more than a launch.  (Two passes over memory, one element a thread and step: 8192 columns of one row 11.5 us in front of a product, 2041 x 4096 bfloat16 12.8.)
 constexpr int OP_ROW_E = 32;
 template <typename T, int W>
 static __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void op_quantize_kernel(const T* __restrict__ x, int64_t rows, int cols, int64_t ldx, int8_t* __restrict__ codes, int64_t ldq, float* __restrict__ scale) {
@@ -143,7 +143,7 @@ template <typename TY> struct OpProductArgs {
 // A few tokens: the weights' bytes are what it costs, and they go from memory to the matrix cores' registers directly.  A wavefront has 16 channels
 // x 16 MT tokens (v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l % 16) and a ring of D steps of 64 k on their way; the KS wavefronts of a
 // workgroup share the channels and split k (their int32 sums meet in LDS: exact in any order).  The tokens' codes come from the caches, which costs
-// 4 % of the weights' time a token (128256 x 4096, us: 1 token 85, 4 95, 16 144, 32 197; tiles 88, 92, 98, 102): op_product_piece compares.
+// 4 % of the weights' time a token (128256 x 4096, us: 1 token 83 = 6.3 TB/s, 4 95, 16 144, 32 197; tiles 88, 92, 96, 96): op_streams compares.
 // (Loads past the caches fetch the 128-byte lines twice, half by half: 85 -> 95.  32 or 64 channels a wavefront: 92, 97.)
 template <int KS> struct OpStrip {          // the wavefront's part of a strip of 16 channels
     int lane, wave, r16, kg, n0, s0, cnt;
@@ -262,11 +262,16 @@ static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<
 // quarter, so the matrix cores have that quarter while the next stage's first fragments are read, and it waits for all loads but those that have a
 // stage left to travel.  16-byte chunk c of row r stands at chunk c ^ (r / 2 % 8): the 16 lanes of a read cover the banks once.  Workgroups go to the
 // 8 XCDs in turn; the token tiles of one channel tile run on one XCD, so its weights leave HBM once.
+// What bounds it: 32 x 128 and 64 x 128 tiles the weights (32 tokens, 151936 x 2560: 77 us, 5.05 TB/s); 256 x 256 tiles the matrix cores: a stage takes about
+// the 2048 cycles that its MFMAs issue in, at the 1.3 - 1.5 GHz that the card's power leaves (512 x 128256 x 4096 250 - 310 us from card to card, 2.1 POP/s with
+// the 1.5 - 4 us in front of a tile's first stage and the 3.3 (bfloat16) - 4.8 us (float32) of its results; a loop of nothing but these MFMAs 4.0).
+// Tried: 64 k a stage with a longer ring of weights, loads by some wavefronts and MFMAs by others (62 -> 85 us at 512 x 28672 x 4096); four wavefronts of
+// 128 x 128 (same); one workgroup a CU that goes through its tiles without a pause (same); priorities, one or three reads behind an MFMA (same).
 __device__ __forceinline__ void op_dma16(const void* src, void* lds) {
     __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src, (__attribute__((address_space(3))) void*)lds, 16, 0, 0);
 }
-// all but the newest N loads of this wavefront have landed, its LDS reads are done, and so are everybody's
 template <int I, int N, typename F> __device__ __forceinline__ void op_static_for(F f) { if constexpr (I < N) { f(std::integral_constant<int, I>{}); op_static_for<I + 1, N>(f); } }
+// all but the newest N loads of this wavefront have landed, its LDS reads are done, and so are everybody's
 template <int N> __device__ __forceinline__ void op_wait_barrier() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" :: "n"(N) : "memory"); }
 
 // TY = int: part blockIdx.y of gridDim.y of the sum over k, y[part][m][ldy] (op_parts_kernel adds them up).

@@ -99,6 +99,24 @@ def test_more_rows_of_logits_than_a_launch_takes(ops):
     assert torch.allclose(got.top_logprobs[:, 0].double(), lp.max(1).values, rtol=0, atol=1e-5)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("vocab", [40, 3001, 40000])
+def test_nan_of_every_kind(ops, dtype, vocab):
+    """Quiet and signalling NaN, of either sign, beside the largest logits: no alternative, and the others' order is what it is without them."""
+    x = torch.from_numpy((rng(vocab).standard_normal((8, vocab)) * 3).astype(np.float32)).to(NAMES[dtype])
+    whole, kinds = {"f32": (torch.int32, [0x7fc00000, 0x7f800001, -0x400000, -0x7fffff]), "f16": (torch.int16, [0x7e00, 0x7c01, -0x200, -0x3ff]), "bf16": (torch.int16, [0x7fc0, 0x7f81, -0x40, -0x7f])}[dtype]
+    bits = x.view(whole)
+    for r in range(8):
+        for i, at in enumerate(torch.topk(x[r].float(), 12).indices.tolist()):
+            if i % 2 and at ^ 1 < vocab:
+                bits[r, at ^ 1] = kinds[(r + i) % 4]          # beside a large one, in its vector
+        bits[r, r] = kinds[r % 4]
+    assert torch.isnan(x).any(1).all()
+    x = x.to(DEV)
+    t = targets_of(8, vocab, 3)
+    check_rows(ops.token_logprobs(x, t, 11), x, t, 11)
+
+
 # ---- offsets that pass 32 bits: the last rows are what they are on their own ----
 def test_results_past_32_bits(ops):
     m, n = 16800, 128256          # 2.15 G results
