@@ -40,6 +40,8 @@ class Int8Rows:
             raise _bad("a row of codes is %d columns and zeros up to a multiple of %d, at most %d" % (cols, CODE_BLOCK, MAX_K))
         if scale.dim() != 1 or scale.shape[0] != codes.shape[0] or scale.dtype != torch.float32 or scale.device != codes.device or not scale.is_contiguous():
             raise _bad("scale must hold one float32 per row of codes, beside them")
+        if scale.requires_grad:
+            raise _bad("scale requires a gradient: these operators are forward only")
         self.codes, self.scale, self.cols = codes, scale, cols
         self.rows, self.device = codes.shape[0], codes.device
         self.ld = codes.stride(0) if self.rows > 1 else codes.shape[1] // 16 * 16
@@ -130,8 +132,12 @@ def _result(w, bias, m, k, dtype, out, device):
         raise _bad("results are float32, float16 or bfloat16")
     if bias is not None:
         _like(bias, "bias", (n,), torch.float32, device)
+        if bias.requires_grad and torch.is_grad_enabled():
+            raise _bad("bias requires a gradient: these operators are forward only")
     if out is None:
         return torch.empty(m, n, dtype=dtype, device=device), n
+    if out.requires_grad and torch.is_grad_enabled():
+        raise _bad("out requires a gradient: these operators are forward only")
     if out.shape != (m, n) or out.dtype != dtype or out.device != device or (out.stride(1) != 1 and n != 1):
         raise _bad("out must be a %d x %d matrix of %s with contiguous rows on %s" % (m, n, dtype, device))
     return out, out.stride(0)

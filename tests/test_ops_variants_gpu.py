@@ -214,3 +214,14 @@ def test_two_graphs_with_workspaces_of_their_own(ops):
         torch.cuda.synchronize()
         for got, ref in zip(outs, want):
             assert torch.equal(got.top_ids, ref.top_ids) and torch.equal(got.top_logprobs, ref.top_logprobs) and torch.equal(got.entropy, ref.entropy)
+
+
+def test_no_gradient_is_lost_in_silence(ops, hip):
+    w, x = int8_rows(ops, 10, 100, 1), torch.randn(4, 100, device=DEV)
+    bias, out = torch.zeros(10, device=DEV, requires_grad=True), torch.zeros(4, 10, device=DEV, requires_grad=True)
+    for call in (lambda: ops.int8_linear(x, w, bias), lambda: ops.int8_matmul(ops.quantize_rows(x), w, bias), lambda: ops.int8_linear(x, w, out=out),
+                 lambda: ops.Int8Rows(w.codes, w.scale.clone().requires_grad_(), 100), lambda: ops.token_logprobs(out), lambda: ops.quantize_rows(out)):
+        with pytest.raises(hip.Gl3Error):
+            call()
+    with torch.no_grad():
+        assert torch.equal(ops.int8_linear(x, w, bias, out=out), ops.int8_linear(x, w))
