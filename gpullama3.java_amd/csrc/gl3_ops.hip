@@ -127,22 +127,27 @@ uint64_t op_product_workspace(int64_t m, int64_t n, int32_t k) {
     return most;
 }
 
-constexpr int OP_TOKEN_STRIPS = 2048;
+constexpr int OP_TOKEN_STRIPS = 2048;          // of one or two tokens; of four half as many, of eight a quarter
 // workspace of a linear: codes of the rows, their scales, then what the product needs
 static uint64_t op_linear_codes(int64_t m, int32_t k) { return (uint64_t)m * op_code_ld(k); }
 static uint64_t op_linear_rows(int64_t m, int32_t k) { return op_linear_codes(m, k) + (uint64_t)op_cdiv(m, 4) * 16; }
-// one token whose row every workgroup quantises for itself: no workspace
-static bool op_token(int64_t m, int64_t n, int32_t k) { return m == 1 && n <= 16 * OP_TOKEN_STRIPS && k <= OP_ROW_E * 512; }
+// a few tokens whose rows every workgroup quantises for itself: no workspace.  lg: 2^lg rows at least
+static int op_token_lg(int64_t m) { return m <= 1 ? 0 : m <= 2 ? 1 : m <= 4 ? 2 : 3; }
+static bool op_token(int64_t m, int64_t n, int32_t k) {
+    const int lg = op_token_lg(m);
+    return m <= OP_TOKENS && n <= 16 * (OP_TOKEN_STRIPS >> std::max(0, lg - 1)) && op_code_ld(k) <= OP_ROW_E * 512 >> lg;
+}
 uint64_t op_linear_workspace(int64_t m, int64_t n, int32_t k) { return op_token(m, n, k) ? 0 : op_linear_rows(m, k) + op_product_workspace(m, n, k); }
 void op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const OpProduct& p, void* workspace) {
     if (op_token(p.m, p.n, p.k)) {
         op_with_type(x_type, [&](auto tx) {
             op_with_type(p.y_type, [&](auto ty) {
                 typedef decltype(tx) TX; typedef decltype(ty) TY;
-                const OpProductArgs<TY> a{nullptr, 0, nullptr, p.w, p.ldw, p.w_scale, p.bias, 1, (int)p.n, (int)op_code_ld(p.k), (TY*)p.y, p.ldy};
+                const OpProductArgs<TY> a{nullptr, 0, nullptr, p.w, p.ldw, p.w_scale, p.bias, (int)p.m, (int)p.n, (int)op_code_ld(p.k), (TY*)p.y, p.ldy};
                 const dim3 grid((unsigned)op_cdiv(p.n, 16));
-                if (grid.x <= OP_FEW_STRIPS || p.k > OP_ROW_E * 256) hipLaunchKernelGGL((op_token_kernel<TX, TY, 8, 4>), grid, dim3(512), 0, s, a, (const TX*)x, p.k);
-                else hipLaunchKernelGGL((op_token_kernel<TX, TY, 4, 8>), grid, dim3(256), 0, s, a, (const TX*)x, p.k);
+                const int lg = op_token_lg(p.m);
+                if (grid.x <= OP_FEW_STRIPS || 4 >> lg == 0 || a.kp > OP_ROW_E * 256 >> lg) hipLaunchKernelGGL((op_token_kernel<TX, TY, 8, 4>), grid, dim3(512), 0, s, a, (const TX*)x, ldx, p.k, lg);
+                else hipLaunchKernelGGL((op_token_kernel<TX, TY, 4, 8>), grid, dim3(256), 0, s, a, (const TX*)x, ldx, p.k, lg);
             });
         });
         return;

@@ -35,15 +35,15 @@ __device__ __forceinline__ int op_code(float v, float to_code) {
     return to_code == 0.f ? 0 : (int)__builtin_rintf(fminf(fmaxf(v * to_code, -127.f), 127.f));
 }
 
-// A thread's share of a row in registers: NV pieces of 16 bytes, NT pieces apart; zeros behind the row's end.
-template <typename T, int NV, int NT> struct OpRowPart {
+// A thread's share of a row in registers: NV pieces of 16 bytes, nt (the threads of a row) pieces apart; zeros behind the row's end.
+template <typename T, int NV> struct OpRowPart {
     static constexpr int V = 16 / (int)sizeof(T);
     T x[NV][V];
-    __device__ __forceinline__ void load(const T* row, int k, int t) {
+    __device__ __forceinline__ void load(const T* row, int k, int t, int nt) {
         if (((uintptr_t)row & 15) == 0) {
 #pragma unroll
             for (int i = 0; i < NV; ++i) {
-                const int c = (t + NT * i) * V;
+                const int c = (t + nt * i) * V;
                 if (c + V <= k) *reinterpret_cast<uint4*>(x[i]) = *reinterpret_cast<const uint4*>(row + c);
                 else
 #pragma unroll
@@ -53,7 +53,7 @@ template <typename T, int NV, int NT> struct OpRowPart {
 #pragma unroll
             for (int i = 0; i < NV; ++i)
 #pragma unroll
-                for (int e = 0; e < V; ++e) { const int c = (t + NT * i) * V + e; x[i][e] = c < k ? row[c] : op_cast<T>(0.f); }
+                for (int e = 0; e < V; ++e) { const int c = (t + nt * i) * V + e; x[i][e] = c < k ? row[c] : op_cast<T>(0.f); }
         }
     }
     __device__ __forceinline__ uint32_t largest() const {          // of the wavefront
@@ -65,10 +65,10 @@ template <typename T, int NV, int NT> struct OpRowPart {
         for (int d = 32; d; d >>= 1) mag = max(mag, (uint32_t)__shfl_xor((int)mag, d));
         return mag;
     }
-    __device__ __forceinline__ void store(int8_t* codes, int kp, int t, float to_code) const {          // kp: the row's end with its zeros
+    __device__ __forceinline__ void store(int8_t* codes, int kp, int t, int nt, float to_code) const {          // kp: the row's end with its zeros
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            const int c = (t + NT * i) * V;
+            const int c = (t + nt * i) * V;
             if (c >= kp) continue;
             uint32_t w[V / 4];
 #pragma unroll
@@ -87,10 +87,10 @@ static __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void op_quantize_kerne
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), t = threadIdx.x & (64 * W - 1);
     const int64_t row = (int64_t)blockIdx.x * (W > 4 ? 1 : 4 / W) + wave / W;
     const bool live = row < rows;
-    OpRowPart<T, OP_ROW_E * (int)sizeof(T) / 16, 64 * W> part;
+    OpRowPart<T, OP_ROW_E * (int)sizeof(T) / 16> part;
     uint32_t mag = 0;
     if (live) {
-        part.load(x + row * ldx, cols, t);
+        part.load(x + row * ldx, cols, t, 64 * W);
         mag = part.largest();
     }
     if constexpr (W > 1) {
@@ -104,7 +104,7 @@ static __global__ __launch_bounds__(W > 4 ? 64 * W : 256) void op_quantize_kerne
     float s, r;
     op_row_scale(mag, s, r);
     if (t == 0) scale[row] = s;
-    part.store(codes + row * ldq, (cols + GL3_CODE_BLOCK - 1) / GL3_CODE_BLOCK * GL3_CODE_BLOCK, t, r);
+    part.store(codes + row * ldq, (cols + GL3_CODE_BLOCK - 1) / GL3_CODE_BLOCK * GL3_CODE_BLOCK, t, 64 * W, r);
 }
 // longer rows: read twice
 template <typename T>
@@ -113,9 +113,9 @@ static __global__ __launch_bounds__(1024) void op_quantize_long_kernel(const T* 
     constexpr int STEP = OP_ROW_E / 2 * 1024;
     const T* row = x + (int64_t)blockIdx.x * ldx;
     const int kp = (cols + GL3_CODE_BLOCK - 1) / GL3_CODE_BLOCK * GL3_CODE_BLOCK;
-    OpRowPart<T, OP_ROW_E / 2 * (int)sizeof(T) / 16, 1024> part;
+    OpRowPart<T, OP_ROW_E / 2 * (int)sizeof(T) / 16> part;
     uint32_t mag = 0;
-    for (int c = 0; c < cols; c += STEP) { part.load(row + c, cols - c, threadIdx.x); mag = max(mag, part.largest()); }
+    for (int c = 0; c < cols; c += STEP) { part.load(row + c, cols - c, threadIdx.x, 1024); mag = max(mag, part.largest()); }
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = mag;
     __syncthreads();
 #pragma unroll
@@ -123,7 +123,7 @@ static __global__ __launch_bounds__(1024) void op_quantize_long_kernel(const T* 
     float s, r;
     op_row_scale(mag, s, r);
     if (threadIdx.x == 0) scale[blockIdx.x] = s;
-    for (int c = 0; c < kp; c += STEP) { part.load(row + c, cols - c, threadIdx.x); part.store(codes + (int64_t)blockIdx.x * ldq + c, kp - c, threadIdx.x, r); }
+    for (int c = 0; c < kp; c += STEP) { part.load(row + c, cols - c, threadIdx.x, 1024); part.store(codes + (int64_t)blockIdx.x * ldq + c, kp - c, threadIdx.x, 1024, r); }
 }
 
 // ---- products -------------------------------------------------------------------------------------------------------------------------
@@ -210,32 +210,39 @@ static __global__ __launch_bounds__(64 * KS) void op_stream_kernel(OpProductArgs
     op_store4(p, v, row, st.n0 + 4 * st.kg, p.as[min(row, p.m - 1)]);
 }
 
-// One token of a linear: every workgroup quantises the row for itself (LDS) while its first weights are on their way, and one launch is all.  That costs each
-// of them about a microsecond, more than the launch where they run in many rounds (us, this / a launch of its own for the codes: 2048 x 2048 5.0 / 8.0, 14336 x 4096
-// 15.0 / 18.0, 32000 x 2048 16.6 / 16.9, 128256 x 4096 95 / 89; several strips a workgroup 100).  k <= OP_ROW_E x threads: the row stays in registers.
+// A few tokens of a linear (at most 8): every workgroup quantises the rows for itself (LDS) while its first weights are on their way, and one launch is all.  That
+// costs each of them about a microsecond, more than the launch where they run in many rounds (us, this / a launch of its own for the codes; 1 token: 2048 x 2048 5.0 / 8.0,
+// 14336 x 4096 15.2 / 18.0, 32000 x 2048 15.7 / 16.9, 128256 x 4096 95 / 89; 2: 4096 x 4096 8.0 / 10.7, 32000 x 4096 27.1 / 29.7; 4: 16000 x 2048 10.6 / 12.4,
+// 32000 x 4096 32.4 / 31.3; 8: 8192 x 2048 8.3 / 11.3, 32000 x 2048 20.8 / 17.6; several strips a workgroup 100).  KS >> lg wavefronts have a row each, in registers: k <= OP_ROW_E x their threads.
+constexpr int OP_TOKENS = 8;
 template <typename TX, typename TY, int KS, int D>
-static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<TY> p, const TX* __restrict__ x, int k) {
-    constexpr int NT = 64 * KS;
-    __shared__ __attribute__((aligned(16))) int8_t codes[OP_ROW_E * NT];
+static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<TY> p, const TX* __restrict__ x, int64_t ldx, int k, int lg) {
+    __shared__ __attribute__((aligned(16))) int8_t codes[OP_ROW_E * 64 * KS + OP_TOKENS * 16];          // rows kp + 16 apart
     __shared__ op_v4i sums[KS][64];
     __shared__ uint32_t red[KS];
+    __shared__ float scales[OP_TOKENS];
     const OpStrip<KS> st(p.w, p.ldw, p.n, p.kp);
-    // the row first: loads come back in order, and the weights behind it do not hold it up
-    OpRowPart<TX, OP_ROW_E * (int)sizeof(TX) / 16, NT> part;
-    part.load(x, k, threadIdx.x);
+    const int per = KS >> lg, row = st.wave / per, nt = 64 * per, t = threadIdx.x & (nt - 1);
+    const bool live = row < p.m;
+    // the rows first: loads come back in order, and the weights behind them do not hold them up
+    OpRowPart<TX, OP_ROW_E * (int)sizeof(TX) / 16> part;
+    if (live) part.load(x + row * ldx, k, t, nt);
     op_v4i acc = {0, 0, 0, 0}, fw[D];
 #pragma unroll
     for (int d = 0; d < D; ++d) fw[d] = st.load(max(0, min(d, st.cnt - 1)));
-    uint32_t mag = part.largest();
+    uint32_t mag = live ? part.largest() : 0;
     if (st.lane == 0) red[st.wave] = mag;
     __syncthreads();
-#pragma unroll
-    for (int q = 0; q < KS; ++q) mag = max(mag, red[q]);
-    float scale, to_code;
-    op_row_scale(mag, scale, to_code);
-    part.store(codes, p.kp, threadIdx.x, to_code);
+    for (int q = 0; q < per; ++q) mag = max(mag, red[row * per + q]);
+    if (live) {
+        float scale, to_code;
+        op_row_scale(mag, scale, to_code);
+        if (t == 0) scales[row] = scale;
+        part.store(codes + row * (p.kp + 16), p.kp, t, nt, to_code);
+    }
     __syncthreads();
-    const int8_t* cb = codes + st.s0 * 64 + 16 * st.kg;          // (all 16 token columns are this token)
+    const int mine = min(st.r16, p.m - 1);
+    const int8_t* cb = codes + mine * (p.kp + 16) + st.s0 * 64 + 16 * st.kg;
     if (st.cnt > 0) {
         int s = 0;
         for (; s + D < st.cnt; s += D)
@@ -254,7 +261,7 @@ static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<
     op_v4i v = sums[0][st.lane];
 #pragma unroll
     for (int q = 1; q < KS; ++q) v += sums[q][st.lane];
-    op_store4(p, v, st.r16, st.n0 + 4 * st.kg, scale);
+    op_store4(p, v, st.r16, st.n0 + 4 * st.kg, scales[mine]);
 }
 
 // More tokens: BM tokens x BN channels per workgroup of WM x WN wavefronts, v_mfma_i32_32x32x32_i8.  The operands go straight to LDS (16 bytes a lane, no

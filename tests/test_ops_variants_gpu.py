@@ -69,6 +69,25 @@ def test_one_token(ops, n, k):
         check_product(y, a, w)
 
 
+@pytest.mark.parametrize("m,n,k", [(2, 100, 8192), (2, 100, 8193), (3, 100, 4096), (4, 100, 4097), (5, 100, 2048), (8, 33, 2049), (7, 700, 1), (2, 9001, 4096), (2, 9001, 4097), (4, 9001, 2048),
+                                   (3, 9001, 2049), (8, 9001, 300), (6, 9001, 1000), (8, 32768, 130), (8, 32769, 130), (4, 16384, 130), (4, 16385, 130), (8, 8192, 130), (8, 8193, 130), (9, 100, 300)])
+def test_a_few_tokens(ops, m, n, k):
+    w = int8_rows(ops, n, k, 4)
+    bias = torch.from_numpy(rng(3).standard_normal(n).astype(np.float32)).to(DEV)
+    for t in NAMES.values():
+        x = torch.from_numpy(odd_rows(m, k + 5, k)).to(t).to(DEV)
+        x = torch.where(torch.isfinite(x), x, torch.ones_like(x))
+        x[m - 1, 3 + k // 2] = float("nan")
+        x[0, 4:] = 0 if m > 1 else x[0, 4:]
+        for v in (x[:, 4:k + 4], x[:, 3:k + 3].contiguous()):
+            wide = torch.full((m + 2, n + 3), 3.0, device=DEV)
+            y = ops.int8_linear(v, w, bias, torch.float32, out=wide[1:m + 1, 2:n + 2])
+            a = ops.quantize_rows(v)
+            assert torch.equal(y.nan_to_num(7e30), ops.int8_matmul(a, w, bias).nan_to_num(7e30)) and bool(torch.isnan(y[m - 1]).all()) == bool(torch.isnan(v[m - 1]).any())          # (one column: the NaN lies beside one of the two views)
+            check_product(y[:m - 1], ops.Int8Rows(a.codes[:m - 1], a.scale[:m - 1], k), w, bias)
+            assert (wide[0] == 3).all() and (wide[m + 1] == 3).all() and (wide[:, :2] == 3).all() and (wide[:, n + 2:] == 3).all()
+
+
 @pytest.mark.parametrize("rows,cols", [(3000, 700), (3000, 2048), (3000, 2049), (70, 5000), (70, 8192), (70, 8193), (64, 8192), (3, 9000), (2, 32768), (2, 32769), (3, 512), (3, 513), (5, 2049)])
 def test_codes_of_rows_of_every_length(ops, rows, cols):
     for dtype in NAMES:
