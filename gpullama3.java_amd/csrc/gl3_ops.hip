@@ -38,7 +38,8 @@ void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32
 // Which tile, and into how many parts its sum over k goes: the ones with the least estimated time.  A stage of a BM x BN tile takes a CU 0.00164 (BM + BN) us for
 // its operands' bytes + 0.0000101 BM BN us for its MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 32 x 128 0.30, 64 x 64 0.25), a tile 3 us and its results'
 // bytes at 37 GB/s besides.  256 CUs take the workgroups in rounds; two workgroups of a small tile share a CU; the weights leave memory at 5.4 TB/s.  Tiles that are
-// too few for the CUs get their sums in parts of at least OP_PART_STAGES stages; a launch of its own adds them up, 2.5 us and what it reads (us, in parts / whole,
+// too few for the CUs get their sums in parts of at least OP_PART_STAGES stages; a launch of its own adds them up, 2.5 us (on the host another 3: 4.5 here)
+// and what it reads (us, in parts / whole,
 // m tokens, n x k: 40, 4096 x 4096 10.9 / 12.3 (parts of 8 stages 12.5); 64, 4096 x 14336 17.7 / 36.1; 256 29.5 / 36.0; 64, 1024 x 4096 7.8 / 10.1; 64, 256 x 131000 24 / 254).
 enum { OP_T256x256, OP_T128x256, OP_T128x128, OP_T64x128, OP_T64x64, OP_T32x128, OP_T_COUNT };
 static const struct { int bm, bn, share; } OP_TILES[OP_T_COUNT] = {{256, 256, 1}, {128, 256, 1}, {128, 128, 2}, {64, 128, 2}, {64, 64, 2}, {32, 128, 2}};
@@ -57,7 +58,7 @@ static OpRingPlan op_ring_plan(int m, int n, int kp, int size) {
         if (whole < best.us) best = OpRingPlan{t, 1, whole};
         const int parts = (int)std::min<int64_t>(std::min(256 / tiles, (int64_t)stages / OP_PART_STAGES), OP_MAX_PARTS);
         if (parts < 2 || bn > 128) continue;          // (parts of the larger tiles: 45.2 us, whole 46.1, at 142 tokens, 11037 x 9472)
-        const double part = (double)op_cdiv(stages, parts) * stage + 3.0 + bm * bn * 4 / 37e3, split = std::max(memory, part) + 1e-3 * part + 2.5 + (double)m * n * 4 * parts / 2.5e6;
+        const double part = (double)op_cdiv(stages, parts) * stage + 3.0 + bm * bn * 4 / 37e3, split = std::max(memory, part) + 1e-3 * part + 4.5 + (double)m * n * 4 * parts / 2.5e6;
         if (split < best.us) best = OpRingPlan{t, parts, split};
     }
     return best;
@@ -86,7 +87,7 @@ static void op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile, int par
 // (4096 x 14336 12.6, four of them 14.5), four where they fill the chip (128256 x 4096 85.3, eight 86.5).
 constexpr int OP_FEW_STRIPS = 512;
 static bool op_streams(int m, int n, int kp, const OpRingPlan& ring) {
-    return m <= 32 && 4.0 + std::max((double)n * kp / 6.6e6 * (1.0 + 0.042 * m), kp / 1660.0 * (1.0 + 0.03 * m)) <= ring.us;
+    return m <= 32 && std::max(4.0 + (double)n * kp / 6.6e6 * (1.0 + 0.042 * m), 3.2 + kp / 1660.0 * (1.0 + 0.03 * m)) <= ring.us;
 }
 template <typename TY>
 static void op_product_piece(hipStream_t s, const OpProductArgs<TY>& p, void* workspace) {

@@ -128,7 +128,8 @@ static __global__ __launch_bounds__(1024) void op_quantize_long_kernel(const T* 
 
 // ---- products -------------------------------------------------------------------------------------------------------------------------
 __device__ __forceinline__ float op_result(int acc, float as, float ws) { return ((float)acc * as) * ws; }
-// Results go past the caches: in them they push out weights on their way (64 tokens, 151936 x 2560 float32, us: through / past them 100 / 86; none stored 81).
+// Results in whole lines of 128 bytes go past the caches: in them they push out weights on their way (64 tokens, 151936 x 2560 float32, us: through / past them
+// 100 / 86; none stored 81).  Other rows need the caches, where the halves of a line meet (2000 x 39171, k = 275, float32 96 / 155, bfloat16 76 / 109).
 template <typename TY> __device__ __forceinline__ void op_store_past(TY* p, TY v) {
     if constexpr (sizeof(TY) == 4) __builtin_nontemporal_store(v, p);
     else __builtin_nontemporal_store(__builtin_bit_cast(uint16_t, v), reinterpret_cast<uint16_t*>(p));
@@ -421,8 +422,8 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
     const int mb = m0 + wm * (BM / WM), nb = n0 + wn * (BN / WN);
     const bool whole = m0 + BM <= p.m && n0 + BN <= p.n, biased = p.bias != nullptr;
     const uint32_t lo = ((uint32_t)(4 * kh) * (uint32_t)p.ldy + r32) * (uint32_t)sizeof(TY);
-    auto store = [&](auto all) {
-        constexpr bool ALL = decltype(all)::value;
+    auto store = [&](auto all, auto past) {
+        constexpr bool ALL = decltype(all)::value, PAST = decltype(past)::value;
         float w_[TN], b_[TN];
 #pragma unroll
         for (int j = 0; j < TN; ++j) { const int c = wn * (BN / WN) + j * 32 + r32; w_[j] = PART ? 0.f : lws[c]; b_[j] = PART ? 0.f : lb[c]; }
@@ -442,13 +443,17 @@ static __global__ __launch_bounds__(WM * WN * 64, 1) void op_ring_kernel(OpProdu
                         if constexpr (PART) { if (in) *at = acc[i][j][4 * g + r]; }
                         else {
                             const float x = op_result(acc[i][j][4 * g + r], s4[r], w_[j]);
-                            if (in) op_store_past(at, op_cast<TY>(biased ? x + b_[j] : x));
+                            const TY r_ = op_cast<TY>(biased ? x + b_[j] : x);
+                            if constexpr (PAST) { if (in) op_store_past(at, r_); }
+                            else { if (in) *at = r_; }
                         }
                     }
                 }
             }
     };
-    if (whole) store(std::true_type{}); else store(std::false_type{});
+    if constexpr (PART) { if (whole) store(std::true_type{}, std::false_type{}); else store(std::false_type{}, std::false_type{}); }
+    else if (((uintptr_t)p.y | (uintptr_t)(p.ldy * (int)sizeof(TY))) & 127) { if (whole) store(std::true_type{}, std::false_type{}); else store(std::false_type{}, std::false_type{}); }
+    else { if (whole) store(std::true_type{}, std::true_type{}); else store(std::false_type{}, std::true_type{}); }
 }
 
 // The parts of a product's sums, added up: grid (n / 256, m), a result a thread.
