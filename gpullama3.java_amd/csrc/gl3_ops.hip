@@ -81,13 +81,14 @@ static void op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile, int par
         default: op_ring_launch<TY, 32, 128, 1, 4, 3, 4>(s, p, parts);          // (rings of 2 and 4: 81 us instead of 77 at 32 tokens, 151936 x 2560)
     }
 }
-// Up to 32 tokens may be streamed: 6.6 TB/s of weights, 4.2 % more time a token (us, streamed / tiles; m tokens, n x k: 1, 4096 x 4096 6.5 / 10.3; 16 8.0 / 10.8;
+// Up to 32 tokens (16 where there are many strips: tiles win beyond) may be streamed: 6.6 TB/s of weights, 4.2 % more time a token (us, streamed / tiles; m tokens, n x k: 1, 4096 x 4096 6.5 / 10.3; 16 8.0 / 10.8;
 // 24 9.1 / 11.6; 8, 4096 x 14336 14.6 / 15.9; 16 18.4 / 16.0; 4, 14336 x 4096 15.0 / 14.8; 8 16.5 / 14.8; 8, 32000 x 2048 16.2 / 14.0), and a strip alone takes
-// 26.6 KB a us, 3 % more time a token (16, 2560 x 9728 14.0 / 11.2; 16, 256 x 131000 117 / 21).  Eight wavefronts share the k of a strip where there are few strips
-// (4096 x 14336 12.6, four of them 14.5), four where they fill the chip (128256 x 4096 85.3, eight 86.5).
+// 26.6 KB a us, 3 % more time a token (16, 2560 x 9728 14.0 / 11.2; 16, 256 x 131000 117 / 21), and 0.5 (more than 16 tokens: 1.5) ns of the whole card's time beside
+// its bytes (1, 100000 x 256 13.3 / 10.3; 20 20.7 / 11.6).  Eight wavefronts share the k of a strip where there are few strips (4096 x 14336 12.6, four of them
+// 14.5), four where they fill the chip (128256 x 4096 85.3, eight 86.5).
 constexpr int OP_FEW_STRIPS = 512;
 static bool op_streams(int m, int n, int kp, const OpRingPlan& ring) {
-    return m <= 32 && std::max(4.0 + (double)n * kp / 6.6e6 * (1.0 + 0.042 * m), 3.2 + kp / 1660.0 * (1.0 + 0.03 * m)) <= ring.us;
+    return m <= (n <= 16 * OP_FEW_STRIPS ? 32 : 16) && std::max(4.0 + (double)n * kp / 6.6e6 * (1.0 + 0.042 * m) + n * (m <= 16 ? 3e-5 : 9e-5), 3.2 + kp / 1660.0 * (1.0 + 0.03 * m)) <= ring.us;
 }
 template <typename TY>
 static void op_product_piece(hipStream_t s, const OpProductArgs<TY>& p, void* workspace) {
@@ -96,7 +97,7 @@ static void op_product_piece(hipStream_t s, const OpProductArgs<TY>& p, void* wo
         const unsigned strips = (unsigned)op_cdiv(p.n, 16);
 #define OP_STREAM(MT, KS, D) hipLaunchKernelGGL((op_stream_kernel<TY, MT, KS, D>), dim3(strips), dim3(64 * KS), 0, s, p)
         if (strips <= OP_FEW_STRIPS) { if (p.m <= 16) OP_STREAM(1, 8, 4); else OP_STREAM(2, 8, 4); }
-        else { if (p.m <= 16) OP_STREAM(1, 4, 8); else OP_STREAM(2, 4, 8); }
+        else OP_STREAM(1, 4, 8);
 #undef OP_STREAM
     } else if (ring.parts == 1) op_ring<TY>(s, p, ring.tile, 1);
     else {

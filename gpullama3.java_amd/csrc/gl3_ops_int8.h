@@ -145,7 +145,7 @@ template <typename TY> struct OpProductArgs {
 // x 16 MT tokens (v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l % 16) and a ring of D steps of 64 k on their way; the KS wavefronts of a
 // workgroup share the channels and split k (their int32 sums meet in LDS: exact in any order).  The tokens' codes come from the caches, which costs
 // 4 % of the weights' time a token (128256 x 4096, us: 1 token 83 = 6.3 TB/s, 4 95, 16 144, 32 197; tiles 88, 92, 96, 96): op_streams compares.
-// (Loads past the caches fetch the 128-byte lines twice, half by half: 85 -> 95.  32 or 64 channels a wavefront: 92, 97.)
+// A short k starts no loads that it does not need (100000 x 256, a step a wavefront: 31 -> 13).  (Loads past the caches fetch the 128-byte lines twice, half by half: 85 -> 95.  32 or 64 channels a wavefront: 92, 97.)
 template <int KS> struct OpStrip {          // the wavefront's part of a strip of 16 channels
     int lane, wave, r16, kg, n0, s0, cnt;
     const int8_t* wb;
@@ -192,7 +192,7 @@ static __global__ __launch_bounds__(64 * KS) void op_stream_kernel(OpProductArgs
     };
     if (st.cnt > 0) {
 #pragma unroll
-        for (int d = 0; d < D; ++d) load(d, min(d, st.cnt - 1));
+        for (int d = 0; d < D; ++d) if (d == 0 || d < st.cnt) load(d, d);
         int s = 0;
         for (; s + D < st.cnt; s += D)
 #pragma unroll
@@ -230,7 +230,7 @@ static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<
     if (live) part.load(x + row * ldx, k, t, nt);
     op_v4i acc = {0, 0, 0, 0}, fw[D];
 #pragma unroll
-    for (int d = 0; d < D; ++d) fw[d] = st.load(max(0, min(d, st.cnt - 1)));
+    for (int d = 0; d < D; ++d) if (d == 0 || d < st.cnt) fw[d] = st.load(d);
     uint32_t mag = live ? part.largest() : 0;
     if (st.lane == 0) red[st.wave] = mag;
     __syncthreads();

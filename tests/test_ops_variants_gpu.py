@@ -57,6 +57,14 @@ def test_sums_in_parts(ops, m, n, k):
         assert torch.equal(z, y)
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 8203, 1500), (1, 16411, 2500), (2, 8203, 1537), (4, 9001, 2600), (5, 8203, 2560), (11, 8200, 5000), (16, 8193, 6016), (3, 8192, 4097), (30, 8100, 1100), (18, 300, 384)])
+def test_strips(ops, m, n, k):
+    a, w = int8_rows(ops, m, k, m, extra=32), int8_rows(ops, n, k, n + 1, extra=16)
+    bias = torch.from_numpy(rng(3).standard_normal(n).astype(np.float32)).to(DEV)
+    check_product(ops.int8_matmul(a, w), a, w)
+    check_product(ops.int8_matmul(a, w, bias, torch.float16), a, w, bias)
+
+
 @pytest.mark.parametrize("n,k", [(9001, 130), (9001, 8192), (9001, 8193), (20, 16384), (20, 16385), (32768, 300), (32769, 300), (5, 1)])
 def test_one_token(ops, n, k):
     w = int8_rows(ops, n, k, 4)
