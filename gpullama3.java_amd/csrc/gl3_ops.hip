@@ -148,8 +148,10 @@ void op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const 
                 const OpProductArgs<TY> a{nullptr, 0, nullptr, p.w, p.ldw, p.w_scale, p.bias, (int)p.m, (int)p.n, (int)op_code_ld(p.k), (TY*)p.y, p.ldy};
                 const dim3 grid((unsigned)op_cdiv(p.n, 16));
                 const int lg = op_token_lg(p.m);
-                if (grid.x <= OP_FEW_STRIPS || 4 >> lg == 0 || a.kp > OP_ROW_E * 256 >> lg) hipLaunchKernelGGL((op_token_kernel<TX, TY, 8, 4>), grid, dim3(512), 0, s, a, (const TX*)x, ldx, p.k, lg);
-                else hipLaunchKernelGGL((op_token_kernel<TX, TY, 4, 8>), grid, dim3(256), 0, s, a, (const TX*)x, ldx, p.k, lg);
+#define OP_TOKEN(KS, D, ONE) hipLaunchKernelGGL((op_token_kernel<TX, TY, KS, D, ONE>), grid, dim3(64 * KS), 0, s, a, (const TX*)x, ldx, p.k, lg)
+                if (grid.x <= OP_FEW_STRIPS || 4 >> lg == 0 || a.kp > OP_ROW_E * 256 >> lg) { if (lg) OP_TOKEN(8, 4, false); else OP_TOKEN(8, 4, true); }
+                else { if (lg) OP_TOKEN(4, 8, false); else OP_TOKEN(4, 8, true); }
+#undef OP_TOKEN
             });
         });
         return;

@@ -216,25 +216,29 @@ static __global__ __launch_bounds__(64 * KS) void op_stream_kernel(OpProductArgs
 // 14336 x 4096 15.2 / 18.0, 32000 x 2048 15.7 / 16.9, 128256 x 4096 95 / 89; 2: 4096 x 4096 8.0 / 10.7, 32000 x 4096 27.1 / 29.7; 4: 16000 x 2048 10.6 / 12.4,
 // 32000 x 4096 32.4 / 31.3; 8: 8192 x 2048 8.3 / 11.3, 32000 x 2048 20.8 / 17.6; several strips a workgroup 100).  KS >> lg wavefronts have a row each, in registers: k <= OP_ROW_E x their threads.
 constexpr int OP_TOKENS = 8;
-template <typename TX, typename TY, int KS, int D>
-static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<TY> p, const TX* __restrict__ x, int64_t ldx, int k, int lg) {
+template <typename TX, typename TY, int KS, int D, bool ONE>          // ONE: lg = 0
+static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<TY> p, const TX* __restrict__ x, int64_t ldx, int k, int lg_) {
+    const int lg = ONE ? 0 : lg_;
     __shared__ __attribute__((aligned(16))) int8_t codes[OP_ROW_E * 64 * KS + OP_TOKENS * 16];          // rows kp + 16 apart
     __shared__ op_v4i sums[KS][64];
     __shared__ uint32_t red[KS];
     __shared__ float scales[OP_TOKENS];
     const OpStrip<KS> st(p.w, p.ldw, p.n, p.kp);
-    const int per = KS >> lg, row = st.wave / per, nt = 64 * per, t = threadIdx.x & (nt - 1);
-    const bool live = row < p.m;
+    constexpr int LOG = KS == 8 ? 3 : 2;
+    static_assert(KS == 1 << LOG, "wavefronts");
+    const int row = st.wave >> (LOG - lg), nt = 64 * KS >> lg, t = threadIdx.x & (nt - 1);
+    const bool live = ONE || row < p.m;
     // the rows first: loads come back in order, and the weights behind them do not hold them up
     OpRowPart<TX, OP_ROW_E * (int)sizeof(TX) / 16> part;
     if (live) part.load(x + row * ldx, k, t, nt);
     op_v4i acc = {0, 0, 0, 0}, fw[D];
 #pragma unroll
-    for (int d = 0; d < D; ++d) if (d == 0 || d < st.cnt) fw[d] = st.load(d);
+    for (int d = 0; d < D; ++d) fw[d] = st.load(max(0, min(d, st.cnt - 1)));          // (branches around them hold everything up: 32000 x 2048 15.5 -> 33)
     uint32_t mag = live ? part.largest() : 0;
     if (st.lane == 0) red[st.wave] = mag;
     __syncthreads();
-    for (int q = 0; q < per; ++q) mag = max(mag, red[row * per + q]);
+#pragma unroll
+    for (int q = 0; q < KS; ++q) { const uint32_t v = red[q]; mag = q >> (LOG - lg) == row ? max(mag, v) : mag; }
     if (live) {
         float scale, to_code;
         op_row_scale(mag, scale, to_code);
@@ -242,7 +246,7 @@ static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<
         part.store(codes + row * (p.kp + 16), p.kp, t, nt, to_code);
     }
     __syncthreads();
-    const int mine = min(st.r16, p.m - 1);
+    const int mine = ONE ? 0 : min(st.r16, p.m - 1);
     const int8_t* cb = codes + mine * (p.kp + 16) + st.s0 * 64 + 16 * st.kg;
     if (st.cnt > 0) {
         int s = 0;
