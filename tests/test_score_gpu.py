@@ -167,6 +167,21 @@ def test_the_int8_head_beside_the_head_it_replaces(hy, tmp_path, dtype):
         assert len(b.generate(list(map(int, toks[:5])), 4)) == 4
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_tokens_drawn_from_an_int8_head(hy, tmp_path, dtype):
+    """Greedy tokens, tokens drawn all but coldly and the scores' first alternative are the largest of the logits that a step hands out."""
+    m = noditar.Model(hy, tmp_path, noditar.config([noditar.att(), noditar.ssm()], width=104, vocab=311), 12)
+    toks = noditar.tokens_for(m.cfg, 12)
+    plans_ = [m.plan(dtype, max_batch=16, ctx=64, int8_head=True) for _ in range(4)]
+    step, greedy, cold, score = plans_
+    ss, sc = step.acquire(), score.acquire()
+    for i, t in enumerate(toks):
+        best = int(np.argmax(step.step(ss, [t], i, [0])[0]))
+        assert greedy.forward_decode_sample(int(t), i, 0.0, 0.95, 0.5) == best
+        assert cold.forward_decode_sample(int(t), i, 1e-4, 0.95, 0.5) == best
+        assert score.score(sc, [t], i, [0], None, 1)["top_ids"][0, 0] == best
+
+
 def test_the_run_tool_scores(hy, plans, pkg, tmp_path):
     m = noditar.Model(hy, tmp_path, noditar.config([noditar.att(), noditar.ssm()]), 9)
     toks = noditar.tokens_for(m.cfg, 12)
