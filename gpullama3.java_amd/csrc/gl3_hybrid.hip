@@ -938,8 +938,7 @@ int32_t gl3_hy_finalize(gl3_ctx* ctx) {
         if (!h->head_q) HY_HIP(hipMalloc((void**)&h->head_q, (size_t)V * h->head_ldq));
         if (!h->head_s) HY_HIP(hipMalloc((void**)&h->head_s, (size_t)V * 4));
         if (!h->head_ws) HY_HIP(hipMalloc(&h->head_ws, std::max<uint64_t>(ws, 16)));
-        op_quantize(ctx->stream, h->head.w, h->f32 ? GL3_TYPE_F32 : GL3_TYPE_BF16, V, W, h->head.ld, h->head_q, h->head_ldq, h->head_s);
-        HY_HIP(hipGetLastError());
+        HY_HIP(op_quantize(ctx->stream, h->head.w, h->f32 ? GL3_TYPE_F32 : GL3_TYPE_BF16, V, W, h->head.ld, h->head_q, h->head_ldq, h->head_s));
         HY_HIP(hipStreamSynchronize(ctx->stream));
         HY_HIP(hipFree(h->head.w));
         h->head.w = nullptr;

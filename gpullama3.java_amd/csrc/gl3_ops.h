@@ -1,4 +1,5 @@
-// gl3_ops.h — the operators on device memory as the library's own plans launch them: arguments checked by the caller, nothing but launches.
+// gl3_ops.h — the operators on device memory as the library's own plans launch them: arguments checked by the caller, nothing but launches.  What fails is the
+// first launch that failed; none follows it.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -20,7 +21,7 @@ struct OpLogprobs {
 uint64_t op_product_workspace(int64_t m, int64_t n, int32_t k);
 uint64_t op_linear_workspace(int64_t m, int64_t n, int32_t k);
 uint64_t op_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top);
-void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale);
-void op_product(hipStream_t s, const OpProduct& p, void* workspace);
-void op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const OpProduct& p, void* workspace);          // p.a, lda, a_scale: not read
-void op_logprobs(hipStream_t s, const OpLogprobs& p, void* workspace);
+hipError_t op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale);
+hipError_t op_product(hipStream_t s, const OpProduct& p, void* workspace);
+hipError_t op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const OpProduct& p, void* workspace);          // p.a, lda, a_scale: not read
+hipError_t op_logprobs(hipStream_t s, const OpLogprobs& p, void* workspace);

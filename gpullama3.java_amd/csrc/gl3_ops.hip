@@ -3,7 +3,9 @@
 
 #include <algorithm>
 #include <climits>
+#include <tuple>
 #include <type_traits>
+#include <utility>
 
 #include "gl3_ops_int8.h"
 #include "gl3_ops_logprobs.h"
@@ -12,26 +14,37 @@ void gl3_set_create_error(const char* msg);
 
 static inline int64_t op_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int64_t OP_GRID = 1 << 22;          // workgroups of one launch, at most (a launch has fewer than 2^32 threads)
-template <typename F> static void op_with_type(int32_t type, F&& f) {
-    if (type == GL3_TYPE_F32) f(float{}); else if (type == GL3_TYPE_F16) f(__half{}); else f(op_bf16{});
+template <typename F> static hipError_t op_with_type(int32_t type, F&& f) {
+    return type == GL3_TYPE_F32 ? f(float{}) : type == GL3_TYPE_F16 ? f(__half{}) : f(op_bf16{});
 }
+// A launch and its own error: what hipGetLastError() holds may be another call's, which the caller has dealt with.  Nothing is launched behind one that failed.
+template <typename... P, size_t... I> static hipError_t op_launch_args(const void* kernel, dim3 grid, dim3 block, hipStream_t s, std::tuple<P...>& v, std::index_sequence<I...>) {
+    void* args[] = {&std::get<I>(v)...};
+    return hipLaunchKernel(kernel, grid, block, args, 0, s);
+}
+template <typename... P, typename... A> static hipError_t op_launch(void (*kernel)(P...), dim3 grid, dim3 block, hipStream_t s, A&&... a) {
+    std::tuple<P...> v(std::forward<A>(a)...);
+    return op_launch_args((const void*)kernel, grid, block, s, v, std::index_sequence_for<P...>{});
+}
+#define OP_TRY(call) do { const hipError_t e_ = (call); if (e_ != hipSuccess) return e_; } while (0)
 
 // ---- launches -------------------------------------------------------------------------------------------------------------------------
-void op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale) {
-    op_with_type(type, [&](auto t) {
+hipError_t op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale) {
+    return op_with_type(type, [&](auto t) {
         typedef decltype(t) T;
         const int64_t kp = op_code_ld(cols);
         for (int64_t r = 0; r < rows; r += OP_GRID) {
             const int64_t n = std::min<int64_t>(OP_GRID, rows - r);
             const T* xr = (const T*)x + r * ldx;
-#define OP_Q(W) hipLaunchKernelGGL((op_quantize_kernel<T, W>), dim3((unsigned)(W > 4 ? n : op_cdiv(n * W, 4))), dim3(W > 4 ? 64 * W : 256), 0, s, xr, n, cols, ldx, codes + r * ldq, ldq, scale + r)
+#define OP_Q(W) OP_TRY(op_launch(op_quantize_kernel<T, W>, dim3((unsigned)(W > 4 ? n : op_cdiv(n * W, 4))), dim3(W > 4 ? 64 * W : 256), s, xr, n, cols, ldx, codes + r * ldq, ldq, scale + r))
             // as many wavefronts a row as it needs; of a few rows more, so that a thread has 16 bytes or so
             if (kp <= 512 || (kp <= OP_ROW_E * 64 && rows > 2048)) OP_Q(1);
             else if (kp <= OP_ROW_E * 256 && (kp <= 2048 || rows > 64)) OP_Q(4);
             else if (kp <= OP_ROW_E * 1024) OP_Q(16);
-            else hipLaunchKernelGGL((op_quantize_long_kernel<T>), dim3((unsigned)n), dim3(1024), 0, s, xr, cols, ldx, codes + r * ldq, ldq, scale + r);
+            else OP_TRY(op_launch(op_quantize_long_kernel<T>, dim3((unsigned)n), dim3(1024), s, xr, cols, ldx, codes + r * ldq, ldq, scale + r));
 #undef OP_Q
         }
+        return hipSuccess;
     });
 }
 
@@ -64,21 +77,21 @@ static OpRingPlan op_ring_plan(int m, int n, int kp, int size) {
     return best;
 }
 template <typename TY, int BM, int BN, int WM, int WN, int SA, int SW>
-static void op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p, int parts) {
+static hipError_t op_ring_launch(hipStream_t s, const OpProductArgs<TY>& p, int parts) {
     const int mt = (int)op_cdiv(p.m, BM), nt = (int)op_cdiv(p.n, BN);
-    hipLaunchKernelGGL((op_ring_kernel<TY, BM, BN, WM, WN, SA, SW>), dim3((unsigned)op_cdiv((int64_t)mt * nt, 8) * 8, (unsigned)parts), dim3(WM * WN * 64), 0, s, p, mt, nt);
+    return op_launch(op_ring_kernel<TY, BM, BN, WM, WN, SA, SW>, dim3((unsigned)op_cdiv((int64_t)mt * nt, 8) * 8, (unsigned)parts), dim3(WM * WN * 64), s, p, mt, nt);
 }
 template <typename TY>
-static void op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile, int parts) {
+static hipError_t op_ring(hipStream_t s, const OpProductArgs<TY>& p, int tile, int parts) {
     if constexpr (!std::is_same<TY, int>::value) {          // (tiles that are never in parts)
         if (tile == OP_T256x256) return op_ring_launch<TY, 256, 256, 4, 2, 2, 3>(s, p, parts);
         if (tile == OP_T128x256) return op_ring_launch<TY, 128, 256, 2, 4, 2, 4>(s, p, parts);
     }
     switch (tile) {
-        case OP_T128x128: op_ring_launch<TY, 128, 128, 2, 2, 2, 3>(s, p, parts); break;
-        case OP_T64x128: op_ring_launch<TY, 64, 128, 2, 2, 2, 4>(s, p, parts); break;
-        case OP_T64x64: op_ring_launch<TY, 64, 64, 2, 2, 4, 5>(s, p, parts); break;
-        default: op_ring_launch<TY, 32, 128, 1, 4, 3, 4>(s, p, parts);          // (rings of 2 and 4: 81 us instead of 77 at 32 tokens, 151936 x 2560)
+        case OP_T128x128: return op_ring_launch<TY, 128, 128, 2, 2, 2, 3>(s, p, parts);
+        case OP_T64x128: return op_ring_launch<TY, 64, 128, 2, 2, 2, 4>(s, p, parts);
+        case OP_T64x64: return op_ring_launch<TY, 64, 64, 2, 2, 4, 5>(s, p, parts);
+        default: return op_ring_launch<TY, 32, 128, 1, 4, 3, 4>(s, p, parts);          // (rings of 2 and 4: 81 us instead of 77 at 32 tokens, 151936 x 2560)
     }
 }
 // Up to 32 tokens (16 where there are many strips: tiles win beyond) may be streamed: 6.6 TB/s of weights, 4.2 % more time a token (us, streamed / tiles; m tokens, n x k: 1, 4096 x 4096 6.5 / 10.3; 16 8.0 / 10.8;
@@ -91,28 +104,28 @@ static bool op_streams(int m, int n, int kp, const OpRingPlan& ring) {
     return m <= (n <= 16 * OP_FEW_STRIPS ? 32 : 16) && std::max(4.0 + (double)n * kp / 6.6e6 * (1.0 + 0.042 * m) + n * (m <= 16 ? 3e-5 : 9e-5), 3.2 + kp / 1660.0 * (1.0 + 0.03 * m)) <= ring.us;
 }
 template <typename TY>
-static void op_product_piece(hipStream_t s, const OpProductArgs<TY>& p, void* workspace) {
+static hipError_t op_product_piece(hipStream_t s, const OpProductArgs<TY>& p, void* workspace) {
     const OpRingPlan ring = op_ring_plan(p.m, p.n, p.kp, sizeof(TY));
     if (op_streams(p.m, p.n, p.kp, ring)) {
         const unsigned strips = (unsigned)op_cdiv(p.n, 16);
-#define OP_STREAM(MT, KS, D) hipLaunchKernelGGL((op_stream_kernel<TY, MT, KS, D>), dim3(strips), dim3(64 * KS), 0, s, p)
+#define OP_STREAM(MT, KS, D) return op_launch(op_stream_kernel<TY, MT, KS, D>, dim3(strips), dim3(64 * KS), s, p)
         if (strips <= OP_FEW_STRIPS) { if (p.m <= 16) OP_STREAM(1, 8, 4); else OP_STREAM(2, 8, 4); }
         else OP_STREAM(1, 4, 8);
 #undef OP_STREAM
-    } else if (ring.parts == 1) op_ring<TY>(s, p, ring.tile, 1);
-    else {
-        op_ring<int>(s, OpProductArgs<int>{p.a, p.lda, nullptr, p.w, p.ldw, nullptr, nullptr, p.m, p.n, p.kp, (int*)workspace, p.n}, ring.tile, ring.parts);
-        hipLaunchKernelGGL((op_parts_kernel<TY>), dim3((unsigned)op_cdiv(p.n, 256), (unsigned)p.m), dim3(256), 0, s, (const int*)workspace, ring.parts, p);
     }
+    if (ring.parts == 1) return op_ring<TY>(s, p, ring.tile, 1);
+    OP_TRY(op_ring<int>(s, OpProductArgs<int>{p.a, p.lda, nullptr, p.w, p.ldw, nullptr, nullptr, p.m, p.n, p.kp, (int*)workspace, p.n}, ring.tile, ring.parts));
+    return op_launch(op_parts_kernel<TY>, dim3((unsigned)op_cdiv(p.n, 256), (unsigned)p.m), dim3(256), s, (const int*)workspace, ring.parts, p);
 }
 constexpr int64_t OP_PM = 1 << 16, OP_PN = 1 << 18;          // a launch's rows and channels: its tiles have 32-bit numbers
-void op_product(hipStream_t s, const OpProduct& p, void* workspace) {
-    op_with_type(p.y_type, [&](auto t) {
+hipError_t op_product(hipStream_t s, const OpProduct& p, void* workspace) {
+    return op_with_type(p.y_type, [&](auto t) {
         typedef decltype(t) TY;
         for (int64_t n = 0; n < p.n; n += OP_PN)
             for (int64_t m = 0; m < p.m; m += OP_PM)
-                op_product_piece(s, OpProductArgs<TY>{p.a + m * p.lda, p.lda, p.a_scale + m, p.w + n * p.ldw, p.ldw, p.w_scale + n, p.bias ? p.bias + n : nullptr, (int)std::min(OP_PM, p.m - m),
-                                                      (int)std::min(OP_PN, p.n - n), (int)op_code_ld(p.k), (TY*)p.y + m * p.ldy + n, p.ldy}, workspace);
+                OP_TRY(op_product_piece(s, OpProductArgs<TY>{p.a + m * p.lda, p.lda, p.a_scale + m, p.w + n * p.ldw, p.ldw, p.w_scale + n, p.bias ? p.bias + n : nullptr, (int)std::min(OP_PM, p.m - m),
+                                                      (int)std::min(OP_PN, p.n - n), (int)op_code_ld(p.k), (TY*)p.y + m * p.ldy + n, p.ldy}, workspace));
+        return hipSuccess;
     });
 }
 // the parts of the piece that needs most (whatever the results' type); pieces run one after the other
@@ -140,28 +153,27 @@ static bool op_token(int64_t m, int64_t n, int32_t k) {
     return m <= OP_TOKENS && n <= 16 * (OP_TOKEN_STRIPS >> std::max(0, lg - 1)) && op_code_ld(k) <= OP_ROW_E * 512 >> lg;
 }
 uint64_t op_linear_workspace(int64_t m, int64_t n, int32_t k) { return op_token(m, n, k) ? 0 : op_linear_rows(m, k) + op_product_workspace(m, n, k); }
-void op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const OpProduct& p, void* workspace) {
+hipError_t op_linear(hipStream_t s, const void* x, int32_t x_type, int64_t ldx, const OpProduct& p, void* workspace) {
     if (op_token(p.m, p.n, p.k)) {
-        op_with_type(x_type, [&](auto tx) {
-            op_with_type(p.y_type, [&](auto ty) {
+        return op_with_type(x_type, [&](auto tx) {
+            return op_with_type(p.y_type, [&](auto ty) {
                 typedef decltype(tx) TX; typedef decltype(ty) TY;
                 const OpProductArgs<TY> a{nullptr, 0, nullptr, p.w, p.ldw, p.w_scale, p.bias, (int)p.m, (int)p.n, (int)op_code_ld(p.k), (TY*)p.y, p.ldy};
                 const dim3 grid((unsigned)op_cdiv(p.n, 16));
                 const int lg = op_token_lg(p.m);
-#define OP_TOKEN(KS, D, ONE) hipLaunchKernelGGL((op_token_kernel<TX, TY, KS, D, ONE>), grid, dim3(64 * KS), 0, s, a, (const TX*)x, ldx, p.k, lg)
+#define OP_TOKEN(KS, D, ONE) return op_launch(op_token_kernel<TX, TY, KS, D, ONE>, grid, dim3(64 * KS), s, a, (const TX*)x, ldx, p.k, lg)
                 if (grid.x <= OP_FEW_STRIPS || 4 >> lg == 0 || a.kp > OP_ROW_E * 256 >> lg) { if (lg) OP_TOKEN(8, 4, false); else OP_TOKEN(8, 4, true); }
                 else { if (lg) OP_TOKEN(4, 8, false); else OP_TOKEN(4, 8, true); }
 #undef OP_TOKEN
             });
         });
-        return;
     }
     OpProduct q = p;
     int8_t* codes = (int8_t*)workspace;
     float* scale = (float*)(codes + op_linear_codes(p.m, p.k));
     q.a = codes; q.lda = op_code_ld(p.k); q.a_scale = scale;
-    op_quantize(s, x, x_type, p.m, p.k, ldx, codes, q.lda, scale);
-    op_product(s, q, (uint8_t*)workspace + op_linear_rows(p.m, p.k));
+    OP_TRY(op_quantize(s, x, x_type, p.m, p.k, ldx, codes, q.lda, scale));
+    return op_product(s, q, (uint8_t*)workspace + op_linear_rows(p.m, p.k));
 }
 
 // Parts of a row: as many as give the launch OP_LP_WGS workgroups, none shorter than a small batch, at most 64 (one lane each joins them).
@@ -178,20 +190,21 @@ uint64_t op_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top) {
     const OpLpPlan pl = op_lp_plan(rows, vocab);
     return pl.parts == 1 ? 0 : (uint64_t)rows * pl.parts * op_part_bytes(top);
 }
-void op_logprobs(hipStream_t s, const OpLogprobs& p, void* workspace) {
+hipError_t op_logprobs(hipStream_t s, const OpLogprobs& p, void* workspace) {
     const OpRowOut o{p.targets, p.top, p.logprob, p.rank, p.entropy, p.top_ids, p.top_logprobs};
     const OpLpPlan pl = op_lp_plan(p.rows, p.vocab);
-    op_with_type(p.type, [&](auto t) {
+    return op_with_type(p.type, [&](auto t) {
         typedef decltype(t) T;
         constexpr int V = 16 / (int)sizeof(T), NT = OP_LP_THREADS;
         for (int64_t r = 0; r < p.rows; r += 65535) {          // (a grid's y)
             const dim3 grid((unsigned)pl.parts, (unsigned)std::min<int64_t>(65535, p.rows - r));
-#define OP_LP(U, TOP) hipLaunchKernelGGL((op_logprobs_kernel<T, U, TOP>), grid, dim3(NT), 0, s, (const T*)p.logits, p.vocab, p.ld, r, pl.per / V, o, (uint8_t*)workspace)
+#define OP_LP(U, TOP) OP_TRY(op_launch(op_logprobs_kernel<T, U, TOP>, grid, dim3(NT), s, (const T*)p.logits, p.vocab, p.ld, r, pl.per / V, o, (uint8_t*)workspace))
             if (pl.big) { if (p.top) OP_LP(OP_LP_BIG / NT / V, true); else OP_LP(OP_LP_BIG / NT / V, false); }
             else { if (p.top) OP_LP(OP_LP_SMALL / NT / V, true); else OP_LP(OP_LP_SMALL / NT / V, false); }
 #undef OP_LP
         }
-        if (pl.parts > 1) hipLaunchKernelGGL((op_logprobs_join_kernel<T>), dim3((unsigned)p.rows), dim3(64 * OP_LP_JOIN_WAVES), 0, s, (const T*)p.logits, p.vocab, p.ld, pl.parts, o, (const uint8_t*)workspace);
+        if (pl.parts == 1) return hipSuccess;
+        return op_launch(op_logprobs_join_kernel<T>, dim3((unsigned)p.rows), dim3(64 * OP_LP_JOIN_WAVES), s, (const T*)p.logits, p.vocab, p.ld, pl.parts, o, (const uint8_t*)workspace);
     });
 }
 
@@ -225,9 +238,10 @@ struct OnDevice {
     }
     ~OnDevice() { if (changed) (void)hipSetDevice(before); }
 };
-int32_t launched() {
-    const hipError_t e = hipGetLastError();
-    return e == hipSuccess ? GL3_OK : refuse(e == hipErrorOutOfMemory ? GL3_E_OOM : GL3_E_HIP, hipGetErrorString(e));
+int32_t launched(hipError_t e) {
+    if (e == hipSuccess) return GL3_OK;
+    (void)hipGetLastError();          // (it is told here)
+    return refuse(e == hipErrorOutOfMemory ? GL3_E_OOM : GL3_E_HIP, hipGetErrorString(e));
 }
 int32_t check_product(const OpProduct& p) {
     OP_ARG(p.k >= 1 && p.k <= GL3_INT8_MAX_K, "k out of range (1 .. GL3_INT8_MAX_K)");
@@ -262,8 +276,7 @@ int32_t gl3_quantize_rows(int32_t device, void* stream, const void* x, int32_t x
     OP_ARG(rows_ok(rows, op_code_ld(cols), ldq), "ldq: a row of codes is cols columns and zeros up to a multiple of GL3_CODE_BLOCK");
     OnDevice on;
     if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
-    op_quantize((hipStream_t)stream, x, x_type, rows, cols, ldx, codes, ldq, scale);
-    return launched();
+    return launched(op_quantize((hipStream_t)stream, x, x_type, rows, cols, ldx, codes, ldq, scale));
 }
 
 int32_t gl3_int8_workspace(int64_t m, int64_t n, int32_t k, uint64_t* matmul_bytes, uint64_t* linear_bytes) {
@@ -285,8 +298,7 @@ int32_t gl3_int8_matmul(int32_t device, void* stream, const int8_t* a, int64_t l
     if ((r = check_workspace(workspace, workspace_bytes, op_product_workspace(m, n, k))) != GL3_OK) return r;
     OnDevice on;
     if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
-    op_product((hipStream_t)stream, p, workspace);
-    return launched();
+    return launched(op_product((hipStream_t)stream, p, workspace));
 }
 
 int32_t gl3_int8_linear(int32_t device, void* stream, const void* x, int32_t x_type, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias, int64_t m, int64_t n,
@@ -300,8 +312,7 @@ int32_t gl3_int8_linear(int32_t device, void* stream, const void* x, int32_t x_t
     if ((r = check_workspace(workspace, workspace_bytes, op_linear_workspace(m, n, k))) != GL3_OK) return r;
     OnDevice on;
     if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
-    op_linear((hipStream_t)stream, x, x_type, ldx, p, workspace);
-    return launched();
+    return launched(op_linear((hipStream_t)stream, x, x_type, ldx, p, workspace));
 }
 
 int32_t gl3_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top, uint64_t* bytes) {
@@ -327,8 +338,7 @@ int32_t gl3_token_logprobs(int32_t device, void* stream, const void* logits, int
     if (!targets && !entropy && top == 0) return GL3_OK;
     OnDevice on;
     if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
-    op_logprobs((hipStream_t)stream, OpLogprobs{logits, type, rows, vocab, ld, targets, top, logprob, rank, entropy, top_ids, top_logprobs}, workspace);
-    return launched();
+    return launched(op_logprobs((hipStream_t)stream, OpLogprobs{logits, type, rows, vocab, ld, targets, top, logprob, rank, entropy, top_ids, top_logprobs}, workspace));
 }
 
 }  // extern "C"

@@ -465,7 +465,7 @@ int32_t gl3_score_enqueue(gl3_ctx* ctx, const gl3_score& s, int first, int rows,
     }
     const OpLogprobs p{logits_dev, GL3_TYPE_F32, rows, ctx->d.vocab, ctx->d.vocab, s.targets ? targets : nullptr, s.top, res, (int32_t*)res + rows, res + 2 * (size_t)rows,
                        (int32_t*)res + 3 * (size_t)rows, res + 3 * (size_t)rows + (size_t)rows * s.top};
-    op_logprobs(ctx->stream, p, scratch);
+    GL3_HIP(op_logprobs(ctx->stream, p, scratch));
     GL3_HIP(hipGetLastError());
     GL3_HIP(hipMemcpyAsync(h + R, res, score_words(rows, s.top) * 4, hipMemcpyDeviceToHost, ctx->stream));
     return GL3_OK;

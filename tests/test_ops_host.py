@@ -164,3 +164,47 @@ def test_an_int8_head_of_what_it_cannot_hold(hip, over):
         setattr(d, k, v)
     out = C.c_void_p()
     assert hip.lib().gl3_create(C.byref(d), C.byref(out)) == hip.E_ARG and b"INT8_HEAD" in hip.lib().gl3_last_error(None)
+
+
+# ---- the host code behind the checks, without a GPU (hip_on_host.py): nothing is followed, launches are counted -------------------------------------
+def test_an_error_of_somebody_else_is_not_an_operators():
+    """A failed call that the program has dealt with leaves an error pending in its thread: operators return what their own launches return, and leave it be."""
+    import hip_on_host
+    hip_on_host.run("""
+    A = 1 << 20
+    calls = [lambda: L.gl3_quantize_rows(0, None, A, 0, 5, 300, 300, A, 384, A),
+             lambda: L.gl3_int8_matmul(0, None, A, 384, A, A, 384, A, None, 5, 70, 300, A, 0, 70, A, 1 << 30),
+             lambda: L.gl3_int8_linear(0, None, A, 0, 300, A, 384, A, None, 5, 70, 300, A, 0, 70, A, 1 << 30),
+             lambda: L.gl3_int8_linear(0, None, A, 0, 300, A, 384, A, None, 500, 70, 300, A, 0, 70, A, 1 << 30),
+             lambda: L.gl3_token_logprobs(0, None, A, 0, 3, 70000, 70000, A, 2, A, A, A, A, A, A, 1 << 30)]
+    for call in calls:
+        assert fake.hipSetDevice(1000) != 0          # pending until somebody asks
+        fake.fake_reset()
+        assert call() == 0, L.gl3_last_error(None)
+        assert fake.fake_launches() >= 1 and fake.fake_pending() != 0
+        fake.hipGetLastError()
+    """)
+
+
+def test_nothing_is_launched_behind_a_launch_that_failed():
+    import hip_on_host
+    hip_on_host.run("""
+    A = 1 << 20
+    calls = [lambda: L.gl3_quantize_rows(0, None, A, 0, 5, 300, 300, A, 384, A),
+             lambda: L.gl3_int8_linear(0, None, A, 0, 300, A, 384, A, None, 500, 70, 300, A, 0, 70, A, 1 << 30),                     # codes, product
+             lambda: L.gl3_int8_linear(0, None, A, 0, 30000, A, 30080, A, None, 40, 300, 30000, A, 0, 300, A, 1 << 30),              # codes, parts, their sums
+             lambda: L.gl3_int8_matmul(0, None, A, 128, A, A, 128, A, None, 200000, 70, 100, A, 0, 70, A, 1 << 30),                  # pieces
+             lambda: L.gl3_token_logprobs(0, None, A, 0, 3, 70000, 70000, A, 2, A, A, A, A, A, A, 1 << 30),                          # parts, join
+             lambda: L.gl3_token_logprobs(0, None, A, 0, 200000, 7, 7, A, 2, A, A, A, A, A, A, 1 << 30)]
+    seen = []
+    for call in calls:
+        fake.fake_reset()
+        assert call() == 0, L.gl3_last_error(None)
+        seen.append(fake.fake_launches())
+        for n in range(1, seen[-1] + 1):
+            fake.fake_reset()
+            fake.fake_fail_launch(n)
+            assert call() == hip.E_HIP and L.gl3_last_error(None)
+            assert fake.fake_launches() == n and fake.fake_pending() == 0, (n, fake.fake_launches())
+    assert seen == [1, 2, 3, 4, 2, 4], seen
+    """)
