@@ -232,6 +232,9 @@ struct gl3_ctx {
         }                                                                                              \
     } while (0)
 
+// An allocation that did not fit is told by the call that made it: it does not stay pending for the launches' check of the next one.
+static inline hipError_t gl3_told(hipError_t e) { if (e != hipSuccess) (void)hipGetLastError(); return e; }
+
 #define GL3_NCCL(call)                                                                                 \
     do {                                                                                               \
         ncclResult_t r_ = (call);                                                                      \

@@ -923,29 +923,32 @@ int32_t gl3_hy_finalize(gl3_ctx* ctx) {
             if ((h->L[l].side->have & need2) != need2) GL3_FAIL(GL3_E_STATE, "layer " + std::to_string(l) + ", second mixer: missing tensors");
         }
     }
+    const bool int8_head = ctx->d.flags & GL3_FLAG_INT8_HEAD;
+    if (int8_head) {          // (a call that failed is made again: everything that can fail stands in front of what must not happen twice)
+        const int V = h->head.rows, W = h->head.k;
+        h->head_ldq = op_code_ld(W);
+        uint64_t ws = 0;
+        for (int m = 1; m <= h->want_cap; ++m) ws = std::max(ws, op_linear_workspace(m, V, W));
+        if (!h->head_q) HY_HIP(gl3_told(hipMalloc((void**)&h->head_q, (size_t)V * h->head_ldq)));
+        if (!h->head_s) HY_HIP(gl3_told(hipMalloc((void**)&h->head_s, (size_t)V * 4)));
+        if (!h->head_ws) HY_HIP(gl3_told(hipMalloc(&h->head_ws, std::max<uint64_t>(ws, 16))));
+        HY_HIP(op_quantize(ctx->stream, h->head.w, h->f32 ? GL3_TYPE_F32 : GL3_TYPE_BF16, V, W, h->head.ld, h->head_q, h->head_ldq, h->head_s));
+        HY_HIP(hipStreamSynchronize(ctx->stream));
+    }
+    HY_HIP(hipDeviceSynchronize());
     if (h->logit_mul != 1.f) {          // the logits' multiplier rides on the final norm's weight
         std::vector<float> w(h->W);
         HY_HIP(hipMemcpy(w.data(), h->final_norm, (size_t)h->W * 4, hipMemcpyDeviceToHost));
         for (float& v : w) v *= h->logit_mul;
         HY_HIP(hipMemcpy(h->final_norm, w.data(), (size_t)h->W * 4, hipMemcpyHostToDevice));
     }
-    if (ctx->d.flags & GL3_FLAG_INT8_HEAD) {
-        const int V = h->head.rows, W = h->head.k;
-        const size_t es = h->f32 ? 4 : 2;
-        h->head_ldq = op_code_ld(W);
-        uint64_t ws = 0;
-        for (int m = 1; m <= h->want_cap; ++m) ws = std::max(ws, op_linear_workspace(m, V, W));
-        if (!h->head_q) HY_HIP(hipMalloc((void**)&h->head_q, (size_t)V * h->head_ldq));
-        if (!h->head_s) HY_HIP(hipMalloc((void**)&h->head_s, (size_t)V * 4));
-        if (!h->head_ws) HY_HIP(hipMalloc(&h->head_ws, std::max<uint64_t>(ws, 16)));
-        HY_HIP(op_quantize(ctx->stream, h->head.w, h->f32 ? GL3_TYPE_F32 : GL3_TYPE_BF16, V, W, h->head.ld, h->head_q, h->head_ldq, h->head_s));
-        HY_HIP(hipStreamSynchronize(ctx->stream));
-        HY_HIP(hipFree(h->head.w));
+    if (int8_head) {
+        (void)hipFree(h->head.w);
         h->head.w = nullptr;
-        h->mat_bytes -= (size_t)V * h->head.ld * es;
-        h->mat_bytes += (size_t)V * h->head_ldq;
+        h->mat_bytes -= (size_t)h->head.rows * h->head.ld * (h->f32 ? 4 : 2);
+        h->mat_bytes += (size_t)h->head.rows * h->head_ldq;
     }
-    HY_HIP(hipDeviceSynchronize());
+    (void)hipDeviceSynchronize();          // (a device that fails here says so in the next call)
     ctx->finalized = true;
     return GL3_OK;
 }
