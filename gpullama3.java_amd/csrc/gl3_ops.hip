@@ -13,7 +13,7 @@
 void gl3_set_create_error(const char* msg);
 
 static inline int64_t op_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
-constexpr int64_t OP_GRID = 1 << 22;          // workgroups of one launch, at most (a launch has fewer than 2^32 threads)
+constexpr int64_t OP_GRID = 1 << 21;          // workgroups of one launch, at most (a launch has fewer than 2^32 threads: 1024 of them a workgroup)
 template <typename F> static hipError_t op_with_type(int32_t type, F&& f) {
     return type == GL3_TYPE_F32 ? f(float{}) : type == GL3_TYPE_F16 ? f(__half{}) : f(op_bf16{});
 }

@@ -208,3 +208,28 @@ def test_nothing_is_launched_behind_a_launch_that_failed():
             assert fake.fake_launches() == n and fake.fake_pending() == 0, (n, fake.fake_launches())
     assert seen == [1, 2, 3, 4, 2, 4], seen
     """)
+
+
+def test_every_launch_has_fewer_threads_than_a_launch_may():
+    """More rows than one launch takes, of every length that the quantiser tells apart: fewer than 2^32 threads a launch, and a workgroup's share for every row."""
+    import hip_on_host
+    hip_on_host.run("""
+    A = 1 << 20
+    for rows in (1, (1 << 21) - 1, 1 << 21, (1 << 21) + 1, 1 << 22, (1 << 23) + 5, 1 << 26):
+        for cols, rows_a_group in ((300, 4), (1500, 4), (5000, 1), (8193, 1), (33000, 1), (131071, 1)):
+            kp = -(-cols // 128) * 128
+            fake.fake_reset()
+            assert L.gl3_quantize_rows(0, None, A, 30, rows, cols, cols, A, kp, A) == 0, (rows, cols, L.gl3_last_error(None))
+            assert fake.fake_most_threads() < 1 << 32 and fake.fake_blocks() * rows_a_group >= rows, (rows, cols)
+    for rows, vocab in ((65536, 9), ((1 << 31) - 1, 9), (1, 1 << 30), (1300, 1 << 30)):
+        fake.fake_reset()
+        assert L.gl3_token_logprobs(0, None, A, 30, rows, vocab, vocab, A, 64, A, A, A, A, A, A, 1 << 62) == 0, (rows, vocab)
+        assert fake.fake_most_threads() < 1 << 32 and fake.fake_blocks() >= rows
+    for m, n, k in ((1 << 24, 5, 9), (5, 1 << 24, 9), (1 << 19, 1 << 19, 131071), (300, 1 << 30, 4096), (1, (1 << 31) - 1, 100), (8, 1 << 20, 2000)):
+        ld = -(-k // 128) * 128
+        fake.fake_reset()
+        ldy = min(n, 1 << 26)
+        r = L.gl3_int8_linear(0, None, A, 30, k, A, ld, A, None, m, n, k, A, 30, n if m == 1 else ldy, A, 1 << 62)
+        assert r == (0 if m == 1 or n <= 1 << 26 else hip.E_ARG), (m, n, k, L.gl3_last_error(None))
+        assert fake.fake_most_threads() < 1 << 32
+    """)
