@@ -448,8 +448,8 @@ int32_t gl3_score_alloc(gl3_ctx* ctx, int rows) {
     uint64_t scratch = 0;
     for (int r = 1; r <= rows; ++r) scratch = std::max(scratch, op_logprobs_workspace(r, ctx->d.vocab, GL3_LOGPROBS_MAX_TOP));
     const size_t words = (size_t)rows + score_words(rows, GL3_LOGPROBS_MAX_TOP);
-    GL3_HIP(hipMalloc(&ctx->sc_dev, (words + 3) / 4 * 16 + scratch));
-    GL3_HIP(hipHostMalloc(&ctx->h_sc, words * 4));
+    GL3_HIP(gl3_told(hipMalloc(&ctx->sc_dev, (words + 3) / 4 * 16 + scratch)));
+    GL3_HIP(gl3_told(hipHostMalloc(&ctx->h_sc, words * 4)));
     ctx->sc_rows = rows;
     return GL3_OK;
 }

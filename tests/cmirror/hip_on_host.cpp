@@ -9,13 +9,14 @@
 
 static thread_local hipError_t g_last = hipSuccess;          // a failed call's error, until somebody asks
 static hipError_t done(hipError_t e) { if (e != hipSuccess) g_last = e; return e; }
-static int g_fail_malloc = 0, g_fail_launch = 0;             // the n-th from now fails
+static int g_fail_malloc = 0, g_fail_host_malloc = 0, g_fail_launch = 0;             // the n-th from now fails
 static uint64_t g_launches = 0, g_most_threads = 0, g_blocks = 0;
 static std::map<void*, size_t> g_held;
 
 extern "C" {
 #define FAKE __attribute__((visibility("default")))
 FAKE void fake_fail_malloc(int n) { g_fail_malloc = n; }
+FAKE void fake_fail_host_malloc(int n) { g_fail_host_malloc = n; }
 FAKE void fake_fail_launch(int n) { g_fail_launch = n; }
 FAKE void fake_reset() { g_launches = g_most_threads = g_blocks = 0; }
 FAKE uint64_t fake_launches() { return g_launches; }
@@ -37,7 +38,11 @@ FAKE hipError_t hipMalloc(void** p, size_t n) {
 }
 FAKE hipError_t hipFree(void* p) { g_held.erase(p); free(p); return hipSuccess; }
 FAKE hipError_t hipExtMallocWithFlags(void** p, size_t n, unsigned) { return hipMalloc(p, n); }
-FAKE hipError_t hipHostMalloc(void** p, size_t n, unsigned) { *p = calloc(1, n ? n : 1); return *p ? hipSuccess : done(hipErrorOutOfMemory); }
+FAKE hipError_t hipHostMalloc(void** p, size_t n, unsigned) {
+    if (g_fail_host_malloc && --g_fail_host_malloc == 0) return done(hipErrorOutOfMemory);
+    *p = calloc(1, n ? n : 1);
+    return *p ? hipSuccess : done(hipErrorOutOfMemory);
+}
 FAKE hipError_t hipHostFree(void* p) { free(p); return hipSuccess; }
 FAKE hipError_t hipMemcpy(void* d, const void* s, size_t n, hipMemcpyKind) { memcpy(d, s, n); return hipSuccess; }
 FAKE hipError_t hipMemcpyAsync(void* d, const void* s, size_t n, hipMemcpyKind, hipStream_t) { memcpy(d, s, n); return hipSuccess; }
