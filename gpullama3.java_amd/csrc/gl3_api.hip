@@ -574,9 +574,15 @@ const char* gl3_version(void) { return "gpullama3-hip 0.1 (gfx950)"; }
 const char* gl3_last_error(gl3_ctx* ctx) { return ctx ? ctx->err.c_str() : create_error(); }
 
 int32_t gl3_create(const gl3_model_desc* desc, gl3_ctx** out) {
+    gl3_no_error();
     if (!desc || !out) { gl3_set_create_error("null argument"); return GL3_E_ARG; }
     if (desc->struct_size != sizeof(gl3_model_desc)) { gl3_set_create_error("gl3_model_desc.struct_size mismatch"); return GL3_E_ARG; }
-    if (desc->arch == GL3_ARCH_NODITAR) { const int32_t r = gl3_hy_create(desc, out, g_create_err); if (r != GL3_OK) publish_create_error(); return r; }
+    if (desc->arch == GL3_ARCH_NODITAR) {
+        std::string why;
+        const int32_t r = gl3_hy_create(desc, out, why);
+        if (r != GL3_OK) gl3_set_create_error(why.c_str());
+        return r;
+    }
     gl3_ctx* ctx = new gl3_ctx();
     ctx->d = *desc;
     ctx->n_seqs = desc->n_seqs < 1 ? 1 : desc->n_seqs;

@@ -16,11 +16,13 @@ const char* gl3_version(void) { return "gpullama3-hip (layer-list family only)";
 const char* gl3_last_error(gl3_ctx* ctx) { return ctx ? ctx->err.c_str() : create_error(); }
 
 int32_t gl3_create(const gl3_model_desc* desc, gl3_ctx** out) {
+    gl3_no_error();
     if (!desc || !out) { gl3_set_create_error("null argument"); return GL3_E_ARG; }
     if (desc->struct_size != sizeof(gl3_model_desc)) { gl3_set_create_error("gl3_model_desc.struct_size mismatch"); return GL3_E_ARG; }
     if (desc->arch != GL3_ARCH_NODITAR) { gl3_set_create_error("this build carries the layer-list family only"); return GL3_E_UNSUPPORTED; }
-    const int32_t r = gl3_hy_create(desc, out, g_create_err);
-    if (r != GL3_OK) publish_create_error();
+    std::string why;
+    const int32_t r = gl3_hy_create(desc, out, why);
+    if (r != GL3_OK) gl3_set_create_error(why.c_str());
     return r;
 }
 

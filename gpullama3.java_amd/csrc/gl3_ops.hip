@@ -10,7 +10,8 @@
 #include "gl3_ops_int8.h"
 #include "gl3_ops_logprobs.h"
 
-void gl3_set_create_error(const char* msg);
+void gl3_set_op_error(const char* msg);          // gl3_create_err.h
+void gl3_no_error();
 
 static inline int64_t op_cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 constexpr int64_t OP_GRID = 1 << 21;          // workgroups of one launch, at most (a launch has fewer than 2^32 threads: 1024 of them a workgroup)
@@ -210,7 +211,7 @@ hipError_t op_logprobs(hipStream_t s, const OpLogprobs& p, void* workspace) {
 
 // ---- entry points ---------------------------------------------------------------------------------------------------------------------
 namespace {
-int32_t refuse(int32_t code, const char* msg) { gl3_set_create_error(msg); return code; }
+int32_t refuse(int32_t code, const char* msg) { gl3_set_op_error(msg); return code; }
 #define OP_ARG(cond, msg) do { if (!(cond)) return refuse(GL3_E_ARG, msg); } while (0)
 
 constexpr int32_t MAX_VOCAB = 1 << 30;
@@ -265,6 +266,7 @@ int32_t check_workspace(const void* workspace, uint64_t have, uint64_t need) {
 extern "C" {
 
 int32_t gl3_quantize_rows(int32_t device, void* stream, const void* x, int32_t x_type, int64_t rows, int32_t cols, int64_t ldx, int8_t* codes, int64_t ldq, float* scale) {
+    gl3_no_error();
     OP_ARG(float_type(x_type), "rows are GL3_TYPE_F32, F16 or BF16");
     OP_ARG(rows >= 0 && rows <= INT32_MAX, "rows out of range");
     OP_ARG(cols >= 1 && cols <= GL3_INT8_MAX_K, "cols out of range (1 .. GL3_INT8_MAX_K)");
@@ -280,6 +282,7 @@ int32_t gl3_quantize_rows(int32_t device, void* stream, const void* x, int32_t x
 }
 
 int32_t gl3_int8_workspace(int64_t m, int64_t n, int32_t k, uint64_t* matmul_bytes, uint64_t* linear_bytes) {
+    gl3_no_error();
     OP_ARG(k >= 1 && k <= GL3_INT8_MAX_K && m >= 0 && n >= 0 && m <= INT32_MAX && n <= INT32_MAX, "sizes out of range");
     const bool none = m == 0 || n == 0;
     if (matmul_bytes) *matmul_bytes = none ? 0 : op_product_workspace(m, n, k);
@@ -289,6 +292,7 @@ int32_t gl3_int8_workspace(int64_t m, int64_t n, int32_t k, uint64_t* matmul_byt
 
 int32_t gl3_int8_matmul(int32_t device, void* stream, const int8_t* a, int64_t lda, const float* a_scale, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias, int64_t m,
                         int64_t n, int32_t k, void* y, int32_t y_type, int64_t ldy, void* workspace, uint64_t workspace_bytes) {
+    gl3_no_error();
     const OpProduct p{a, lda, a_scale, w, ldw, w_scale, bias, m, n, k, y, y_type, ldy};
     int32_t r = check_product(p);
     if (r != GL3_OK || m == 0 || n == 0) return r;
@@ -303,6 +307,7 @@ int32_t gl3_int8_matmul(int32_t device, void* stream, const int8_t* a, int64_t l
 
 int32_t gl3_int8_linear(int32_t device, void* stream, const void* x, int32_t x_type, int64_t ldx, const int8_t* w, int64_t ldw, const float* w_scale, const float* bias, int64_t m, int64_t n,
                         int32_t k, void* y, int32_t y_type, int64_t ldy, void* workspace, uint64_t workspace_bytes) {
+    gl3_no_error();
     const OpProduct p{nullptr, 0, nullptr, w, ldw, w_scale, bias, m, n, k, y, y_type, ldy};
     OP_ARG(float_type(x_type), "rows are GL3_TYPE_F32, F16 or BF16");
     int32_t r = check_product(p);
@@ -316,6 +321,7 @@ int32_t gl3_int8_linear(int32_t device, void* stream, const void* x, int32_t x_t
 }
 
 int32_t gl3_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top, uint64_t* bytes) {
+    gl3_no_error();
     OP_ARG(bytes, "null pointer");
     OP_ARG(rows >= 0 && rows <= INT32_MAX && vocab >= 1 && vocab <= MAX_VOCAB && top >= 0 && top <= GL3_LOGPROBS_MAX_TOP, "sizes out of range");
     *bytes = rows == 0 ? 0 : op_logprobs_workspace(rows, vocab, top);
@@ -324,6 +330,7 @@ int32_t gl3_logprobs_workspace(int64_t rows, int32_t vocab, int32_t top, uint64_
 
 int32_t gl3_token_logprobs(int32_t device, void* stream, const void* logits, int32_t type, int64_t rows, int32_t vocab, int64_t ld, const int32_t* targets, int32_t top, float* logprob,
                            int32_t* rank, float* entropy, int32_t* top_ids, float* top_logprobs, void* workspace, uint64_t workspace_bytes) {
+    gl3_no_error();
     OP_ARG(float_type(type), "logits are GL3_TYPE_F32, F16 or BF16");
     OP_ARG(rows >= 0 && rows <= INT32_MAX && vocab >= 1 && vocab <= MAX_VOCAB, "rows or vocab out of range");
     OP_ARG(top >= 0 && top <= GL3_LOGPROBS_MAX_TOP, "top out of range (0 .. GL3_LOGPROBS_MAX_TOP)");

@@ -562,7 +562,9 @@ GL3_API int32_t gl3_probe_peaks(int32_t device, double* hbm_read_gbs, double* hb
 GL3_API int32_t gl3_get_init_ms(gl3_ctx* ctx, double* plan_ms, double* copy_in_ms);
 
 GL3_API void gl3_destroy(gl3_ctx* ctx);
-GL3_API const char* gl3_last_error(gl3_ctx* ctx);  /* ctx may be NULL: last error without a plan (creating one, operators) of the calling thread */
+GL3_API const char* gl3_last_error(gl3_ctx* ctx);  /* ctx may be NULL: errors of calls without a plan.  An operator's is its
+                                                    * thread's until that thread's next such call; else the newest of any thread, and a
+                                                    * thread whose own plan could not be made reads the newest of making plans */
 
 /* ---- native GGUF loader.  Replaces, for this path, J/tensor/GGUF.java:43-137,217-311 (header,
  * metadata, tensor infos, alignment), the config extraction of LlamaModelLoader.java:47-69 / Qwen3ModelLoader.java:48-79, the
@@ -625,7 +627,7 @@ GL3_API int32_t gl3_profile_hybrid_gemm(int32_t device, int32_t f32, int32_t row
  * into a graph; results and `workspace` (scratch the caller owns, as many bytes as the *_workspace function of the same sizes says, 16-byte
  * aligned, NULL where that is 0) belong to the call until the stream has passed it, so calls that may run at the same time need workspaces of
  * their own, and so do two graphs that may be replayed at the same time.  Outputs must not overlap inputs or each other.  Row strides (ld*) count
- * elements.  0 rows: nothing to do.  Errors: gl3_last_error(NULL), of the calling thread; nothing has been enqueued when arguments are refused. */
+ * elements.  0 rows: nothing to do.  Errors: gl3_last_error(NULL), the calling thread's; nothing has been enqueued when arguments are refused. */
 
 /* rows x cols values of GL3_TYPE_F32 / GL3_TYPE_F16 / GL3_TYPE_BF16 -> int8 codes and one float32 scale per row: x = code * scale within half a
  * step.  With a = max |x| of the row: scale = a / 127, code = rint(x * (127 / a)), every operation rounded to float32 (a code is the same bits

@@ -233,3 +233,30 @@ def test_every_launch_has_fewer_threads_than_a_launch_may():
         assert r == (0 if m == 1 or n <= 1 << 26 else hip.E_ARG), (m, n, k, L.gl3_last_error(None))
         assert fake.fake_most_threads() < 1 << 32
     """)
+
+
+def test_a_plan_that_could_not_be_made_is_told_to_every_thread(hip):
+    """The newest such error, also in a thread that has had one of its own, or an operator's before its last call; an operator's own error stays until then."""
+    import threading
+    L = hip.lib()
+    out = C.c_void_p()
+
+    def elsewhere(call):
+        t = threading.Thread(target=call)
+        t.start()
+        t.join()
+    fails_here = lambda: L.gl3_create(C.byref(hip.ModelDesc()), C.byref(out))          # (no struct_size)
+    fails_there = lambda: L.gl3_create(None, C.byref(out))
+    assert fails_here() == hip.E_ARG and L.gl3_last_error(None) == b"gl3_model_desc.struct_size mismatch"
+    elsewhere(fails_there)
+    assert L.gl3_last_error(None) == b"null argument"
+    assert L.gl3_token_logprobs(*logprobs(top=65)) == hip.E_ARG
+    elsewhere(fails_there)
+    elsewhere(lambda: L.gl3_quantize_rows(*quantize(cols=0)))
+    assert b"top" in L.gl3_last_error(None)
+    assert L.gl3_token_logprobs(*logprobs(rows=0)) == 0
+    elsewhere(fails_there)
+    assert L.gl3_last_error(None) == b"null argument"
+    assert fails_here() == hip.E_ARG
+    elsewhere(lambda: L.gl3_quantize_rows(*quantize(cols=0)))
+    assert L.gl3_last_error(None) == b"gl3_model_desc.struct_size mismatch"
