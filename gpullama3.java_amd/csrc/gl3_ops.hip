@@ -273,7 +273,7 @@ int32_t gl3_quantize_rows(int32_t device, void* stream, const void* x, int32_t x
     if (rows == 0) return GL3_OK;
     OP_ARG(x && codes && scale, "null pointer");
     OP_ARG(aligned(x, type_size(x_type)) && aligned(scale, 4), "misaligned pointer");
-    OP_ARG(rows_ok(rows, cols, ldx), "ldx is less than cols");
+    OP_ARG(rows_ok(rows, cols, ldx), "ldx is less than cols, or rows end past what an address holds");
     OP_ARG(aligned(codes, 16) && ldq % 16 == 0, "codes start on 16 bytes, and so does every row of them");
     OP_ARG(rows_ok(rows, op_code_ld(cols), ldq), "ldq: a row of codes is cols columns and zeros up to a multiple of GL3_CODE_BLOCK");
     OnDevice on;
@@ -298,7 +298,8 @@ int32_t gl3_int8_matmul(int32_t device, void* stream, const int8_t* a, int64_t l
     if (r != GL3_OK || m == 0 || n == 0) return r;
     OP_ARG(a && a_scale, "null pointer");
     OP_ARG(aligned(a, 16) && lda % 16 == 0, "codes start on 16 bytes, and so does every row of them");
-    OP_ARG(rows_ok(m, op_code_ld(k), lda) && lda <= MAX_CODE_LD && aligned(a_scale, 4), "lda: a row of codes is k columns and zeros up to a multiple of GL3_CODE_BLOCK");
+    OP_ARG(aligned(a_scale, 4), "misaligned pointer");
+    OP_ARG(rows_ok(m, op_code_ld(k), lda) && lda <= MAX_CODE_LD, "lda: a row of codes is k columns and zeros up to a multiple of GL3_CODE_BLOCK");
     if ((r = check_workspace(workspace, workspace_bytes, op_product_workspace(m, n, k))) != GL3_OK) return r;
     OnDevice on;
     if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
@@ -313,7 +314,7 @@ int32_t gl3_int8_linear(int32_t device, void* stream, const void* x, int32_t x_t
     int32_t r = check_product(p);
     if (r != GL3_OK || m == 0 || n == 0) return r;
     OP_ARG(x && aligned(x, type_size(x_type)), "x is null or misaligned");
-    OP_ARG(rows_ok(m, k, ldx), "ldx is less than k");
+    OP_ARG(rows_ok(m, k, ldx), "ldx is less than k, or rows end past what an address holds");
     if ((r = check_workspace(workspace, workspace_bytes, op_linear_workspace(m, n, k))) != GL3_OK) return r;
     OnDevice on;
     if (const char* why = on.enter(device, (hipStream_t)stream)) return refuse(GL3_E_ARG, why);
@@ -337,7 +338,7 @@ int32_t gl3_token_logprobs(int32_t device, void* stream, const void* logits, int
     OP_ARG((targets != nullptr) == (logprob != nullptr) && (targets != nullptr) == (rank != nullptr), "targets, logprob and rank: all or none");
     if (rows == 0) return GL3_OK;
     OP_ARG(logits && aligned(logits, type_size(type)), "logits are null or misaligned");
-    OP_ARG(rows_ok(rows, vocab, ld), "ld is less than vocab");
+    OP_ARG(rows_ok(rows, vocab, ld), "ld is less than vocab, or rows end past what an address holds");
     OP_ARG(top == 0 || (top_ids && top_logprobs), "top > 0 needs top_ids and top_logprobs");
     OP_ARG(aligned(targets, 4) && aligned(logprob, 4) && aligned(rank, 4) && aligned(entropy, 4) && aligned(top_ids, 4) && aligned(top_logprobs, 4), "misaligned pointer");
     int32_t r = check_workspace(workspace, workspace_bytes, op_logprobs_workspace(rows, vocab, top));

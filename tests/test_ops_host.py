@@ -260,3 +260,40 @@ def test_a_plan_that_could_not_be_made_is_told_to_every_thread(hip):
     assert fails_here() == hip.E_ARG
     elsewhere(lambda: L.gl3_quantize_rows(*quantize(cols=0)))
     assert L.gl3_last_error(None) == b"gl3_model_desc.struct_size mismatch"
+
+
+WORDS = {"gl3_quantize_rows": dict(type="GL3_TYPE_F32", rows="rows out of range", cols="cols out of range", x="null pointer", codes="null pointer", scale="null pointer", ldx="ldx is less", ldq="ldq",
+                                   device="device"),
+         "gl3_int8_matmul": dict(k="k out of range", m="m or n", n="m or n", y_type="results are", w="null pointer", w_scale="null pointer", y="null pointer", ldw="ldw", ldy="ldy", a="null pointer",
+                                 a_scale="null pointer", lda="lda", device="device"),
+         "gl3_int8_linear": dict(x_type="rows are GL3_TYPE_F32", x="x is null", ldx="ldx is less", workspace="workspace too small", bytes="workspace too small"),
+         "gl3_token_logprobs": dict(type="logits are GL3_TYPE_F32", rows="rows or vocab", vocab="rows or vocab", top="top out of range", targets="all or none", logprob="all or none", rank="all or none",
+                                    logits="logits are null", ld="ld is less", top_ids="top > 0 needs", top_logprobs="top > 0 needs", device="device")}
+WORDS["gl3_int8_linear"] = dict(WORDS["gl3_int8_matmul"], **WORDS["gl3_int8_linear"])
+
+
+def reason(name, kw):
+    """A word of the message that names the first argument of kw (all have one that decides)."""
+    if name == "gl3_int8_matmul" and "k" in kw and ("lda" in kw or "ldw" in kw):          # (the other one is too short then)
+        return "ldw: " if "lda" in kw else "lda: "
+    if name == "gl3_int8_linear" and kw == dict(k=129, ldx=129):
+        return "ldw: "
+    if kw.get("cols") == 131072:
+        return "cols out of range"
+    key, value = next(iter((k, v) for k, v in kw.items() if k not in ("type", "y_type", "x_type", "m") or len(kw) == 1))
+    if key in ("codes", "ldq", "w", "ldw", "a", "lda") and value is not None and value % 16:
+        return "start on 16 bytes"
+    if isinstance(value, int) and value >= A and key in ("x", "scale", "w_scale", "bias", "y", "a_scale", "targets", "logprob", "rank", "entropy", "top_ids", "top_logprobs") and name + key != "gl3_int8_linearx":
+        return "misaligned pointer"
+    if key == "workspace" and value is not None:
+        return "the workspace starts on 16 bytes"
+    return WORDS[name][key]
+
+
+@pytest.mark.parametrize("i", range(len(BAD)))
+def test_a_refusal_names_its_reason(hip, i):
+    name, make, kw = BAD[i]
+    L = hip.lib()
+    assert L.gl3_int8_workspace(0, 0, 0, None, None) == hip.E_ARG and L.gl3_last_error(None) == b"sizes out of range"          # (the message before)
+    assert getattr(L, name)(*make(**kw)) == hip.E_ARG
+    assert reason(name, kw).encode() in L.gl3_last_error(None), (name, kw, L.gl3_last_error(None))
