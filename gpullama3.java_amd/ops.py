@@ -13,6 +13,7 @@ import functools
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import hip
 
@@ -28,6 +29,14 @@ def _bad(what):
 _TYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
 
 
+def _forward_only(t, name):
+    """No derivative is lost in silence, of either mode (no_grad stops gradients only)."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise _bad(name + " requires a gradient: these operators are forward only")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        raise _bad(name + " has a tangent: these operators are forward only")
+
+
 class Int8Rows:
     """Rows of int8 codes with a scale each; row i stands for codes[i, :cols] * scale[i].  codes: int8 [rows, ld], ld >= cols rounded up to a
     multiple of CODE_BLOCK, rows that start on 16 bytes, zeros from column cols to that multiple; scale: float32 [rows].  Checked once, here."""
@@ -40,8 +49,7 @@ class Int8Rows:
             raise _bad("a row of codes is %d columns and zeros up to a multiple of %d, at most %d" % (cols, CODE_BLOCK, MAX_K))
         if scale.dim() != 1 or scale.shape[0] != codes.shape[0] or scale.dtype != torch.float32 or scale.device != codes.device or not scale.is_contiguous():
             raise _bad("scale must hold one float32 per row of codes, beside them")
-        if scale.requires_grad:
-            raise _bad("scale requires a gradient: these operators are forward only")
+        _forward_only(scale, "scale")
         self.codes, self.scale, self.cols = codes, scale, cols
         self.rows, self.device = codes.shape[0], codes.device
         self.ld = codes.stride(0) if self.rows > 1 else codes.shape[1] // 16 * 16
@@ -69,8 +77,7 @@ def _rows(x, name):
     rows, inner = x.stride()
     if inner != 1 and x.shape[1] != 1:
         raise _bad(name + ": the elements of a row must be contiguous")
-    if x.requires_grad and torch.is_grad_enabled():
-        raise _bad(name + " requires a gradient: these operators are forward only")
+    _forward_only(x, name)
     return rows
 
 
@@ -130,14 +137,13 @@ def _result(w, bias, m, k, dtype, out, device):
         raise _bad("the rows have %d columns on %s, the weights %d on %s" % (k, device, w.cols, w.device))
     if dtype not in _TYPES:
         raise _bad("results are float32, float16 or bfloat16")
+    _forward_only(w.scale, "scale")
     if bias is not None:
         _like(bias, "bias", (n,), torch.float32, device)
-        if bias.requires_grad and torch.is_grad_enabled():
-            raise _bad("bias requires a gradient: these operators are forward only")
+        _forward_only(bias, "bias")
     if out is None:
         return torch.empty(m, n, dtype=dtype, device=device), n
-    if out.requires_grad and torch.is_grad_enabled():
-        raise _bad("out requires a gradient: these operators are forward only")
+    _forward_only(out, "out")
     if out.shape != (m, n) or out.dtype != dtype or out.device != device or (out.stride(1) != 1 and n != 1):
         raise _bad("out must be a %d x %d matrix of %s with contiguous rows on %s" % (m, n, dtype, device))
     return out, out.stride(0)
@@ -149,6 +155,7 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None, d
     if device.type != "cuda":
         raise _bad("a must be on a GPU: there is no CPU path")
     m, k, n = a.rows, a.cols, w.rows
+    _forward_only(a.scale, "scale")
     out, ldy = _result(w, bias, m, k, dtype, out, device)
     nbytes = _int8_bytes(m, n, k)[0]
     ws = _workspace(nbytes, device)

@@ -297,3 +297,20 @@ def test_a_refusal_names_its_reason(hip, i):
     assert L.gl3_int8_workspace(0, 0, 0, None, None) == hip.E_ARG and L.gl3_last_error(None) == b"sizes out of range"          # (the message before)
     assert getattr(L, name)(*make(**kw)) == hip.E_ARG
     assert reason(name, kw).encode() in L.gl3_last_error(None), (name, kw, L.gl3_last_error(None))
+
+
+def test_scales_and_their_derivatives(hip, ops):
+    """A scale that requires a gradient is refused where gradients are recorded, and only there; one with a tangent everywhere."""
+    from torch.autograd import forward_ad
+    codes, scale = torch.zeros(3, 128, dtype=torch.int8), torch.ones(3)
+    learned = torch.ones(3, requires_grad=True)
+    with pytest.raises(hip.Gl3Error):
+        ops.Int8Rows(codes, learned, 5)
+    with torch.no_grad():
+        assert ops.Int8Rows(codes, learned, 5).rows == 3
+    with forward_ad.dual_level():
+        with pytest.raises(hip.Gl3Error):
+            ops.Int8Rows(codes, forward_ad.make_dual(scale, torch.ones(3)), 5)
+        with torch.no_grad(), pytest.raises(hip.Gl3Error):
+            ops.Int8Rows(codes, forward_ad.make_dual(scale, torch.ones(3)), 5)
+        assert ops.Int8Rows(codes, scale, 5).rows == 3

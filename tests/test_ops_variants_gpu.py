@@ -252,3 +252,34 @@ def test_no_gradient_is_lost_in_silence(ops, hip):
             call()
     with torch.no_grad():
         assert torch.equal(ops.int8_linear(x, w, bias, out=out), ops.int8_linear(x, w))
+
+
+def test_no_tangent_is_lost_in_silence(ops, hip):
+    """Forward-mode derivatives, of every float input, also where gradients are off; and scales that require a gradient only after they have been wrapped."""
+    from torch.autograd import forward_ad
+    w, x, bias = int8_rows(ops, 10, 100, 1), torch.randn(4, 100, device=DEV), torch.zeros(10, device=DEV)
+    a = ops.quantize_rows(x)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: ops.quantize_rows(dual(x)), lambda: ops.int8_linear(dual(x), w), lambda: ops.int8_linear(x, w, dual(bias)), lambda: ops.int8_matmul(a, w, dual(bias)),
+                     lambda: ops.token_logprobs(dual(x)), lambda: ops.int8_linear(x, w, out=dual(torch.zeros(4, 10, device=DEV))), lambda: ops.Int8Rows(w.codes, dual(w.scale), 100)):
+            with pytest.raises(hip.Gl3Error):
+                call()
+            with torch.no_grad(), pytest.raises(hip.Gl3Error):
+                call()
+        assert torch.equal(ops.int8_linear(x, w), ops.int8_matmul(a, w))          # (nothing here has one)
+    with pytest.raises(hip.Gl3Error):
+        torch.func.jvp(lambda t: ops.token_logprobs(t).entropy, (x,), (x,))
+    want = ops.int8_linear(x, w)
+    for rows in (w, a):
+        rows.scale.requires_grad_()
+        with pytest.raises(hip.Gl3Error):
+            ops.int8_matmul(a, w)
+        with torch.no_grad():
+            assert torch.equal(ops.int8_matmul(a, w), want)
+        rows.scale.requires_grad_(False)
+    w.scale.requires_grad_()
+    with pytest.raises(hip.Gl3Error):
+        ops.int8_linear(x, w)
+    with torch.no_grad():
+        assert torch.equal(ops.int8_linear(x, w), want)
