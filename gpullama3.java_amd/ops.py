@@ -149,6 +149,13 @@ def _result(w, bias, m, k, dtype, out, device):
     return out, out.stride(0)
 
 
+def _written(out):
+    """out= has been written in place: a backward pass that has saved it finds that."""
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
 def int8_matmul(a: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None, dtype=torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """y[i, j] = (sum_k a[i, k] w[j, k]) * a.scale[i] * w.scale[j] (+ bias[j]): the sum exact in int32, one rounding to dtype."""
     device = a.device
@@ -156,12 +163,12 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None, d
         raise _bad("a must be on a GPU: there is no CPU path")
     m, k, n = a.rows, a.cols, w.rows
     _forward_only(a.scale, "scale")
-    out, ldy = _result(w, bias, m, k, dtype, out, device)
+    y, ldy = _result(w, bias, m, k, dtype, out, device)
     nbytes = _int8_bytes(m, n, k)[0]
     ws = _workspace(nbytes, device)
     _call(hip.lib().gl3_int8_matmul, device, a.codes.data_ptr(), a.ld, a.scale.data_ptr(), w.codes.data_ptr(), w.ld, w.scale.data_ptr(), _ptr(bias), m, n, k,
-          out.data_ptr(), _TYPES[dtype], ldy, _ptr(ws), nbytes)
-    return out
+          y.data_ptr(), _TYPES[dtype], ldy, _ptr(ws), nbytes)
+    return y if out is None else _written(out)
 
 
 def int8_linear(x: torch.Tensor, w: Int8Rows, bias: Optional[torch.Tensor] = None, dtype=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -172,12 +179,12 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, bias: Optional[torch.Tensor] = Non
     device = x.device
     if dtype is None:
         dtype = x.dtype
-    out, ldy = _result(w, bias, m, k, dtype, out, device)
+    y, ldy = _result(w, bias, m, k, dtype, out, device)
     nbytes = _int8_bytes(m, n, k)[1]
     ws = _workspace(nbytes, device)
     _call(hip.lib().gl3_int8_linear, device, x.data_ptr(), _TYPES[x.dtype], ldx, w.codes.data_ptr(), w.ld, w.scale.data_ptr(), _ptr(bias), m, n, k,
-          out.data_ptr(), _TYPES[dtype], ldy, _ptr(ws), nbytes)
-    return out
+          y.data_ptr(), _TYPES[dtype], ldy, _ptr(ws), nbytes)
+    return y if out is None else _written(out)
 
 
 def token_logprobs(logits: torch.Tensor, targets: Optional[torch.Tensor] = None, top: int = 0, entropy: bool = True) -> TokenLogprobs:

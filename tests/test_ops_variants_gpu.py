@@ -283,3 +283,18 @@ def test_no_tangent_is_lost_in_silence(ops, hip):
         ops.int8_linear(x, w)
     with torch.no_grad():
         assert torch.equal(ops.int8_linear(x, w), want)
+
+
+def test_a_saved_tensor_that_is_written_is_noticed(ops):
+    """out= is a write in place: a backward pass that has saved the tensor refuses it, as for torch's own."""
+    w, x = int8_rows(ops, 10, 100, 1), torch.randn(4, 100, device=DEV)
+    for call in (lambda out: ops.int8_linear(x, w, out=out), lambda out: ops.int8_matmul(ops.quantize_rows(x), w, out=out)):
+        wide = torch.ones(6, 12, device=DEV)
+        g = torch.ones(6, 12, device=DEV, requires_grad=True)
+        y = (g * wide).sum()          # saves wide
+        call(wide[1:5, 1:11])
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    with torch.inference_mode():
+        out = torch.zeros(4, 10, device=DEV)
+        assert torch.equal(ops.int8_linear(x, w, out=out), ops.int8_linear(x, w))
