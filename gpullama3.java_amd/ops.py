@@ -149,6 +149,25 @@ def _result(w, bias, m, k, dtype, out, device):
     return out, out.stride(0)
 
 
+def _meet(p, p_pitch, p_width, q, q_pitch, q_width, rows):
+    """Whether two matrices of `rows` rows, given by address, bytes between rows and bytes of a row, share a byte (of different pitches: may share one)."""
+    if p + (rows - 1) * p_pitch + p_width <= q or q + (rows - 1) * q_pitch + q_width <= p:
+        return False
+    if rows == 1 or p_pitch != q_pitch:
+        return True
+    gap = (q - p) % p_pitch          # columns of one buffer, side by side
+    return not (p_width <= gap and gap + q_width <= p_pitch)
+
+
+def _apart(out, m, n, ldy, x, ldx, k, bias):
+    """Workgroups write results while others still read: out must not lie over an input."""
+    size, at = out.element_size(), out.data_ptr()
+    if x is not None and _meet(at, ldy * size, n * size, x.data_ptr(), ldx * x.element_size(), k * x.element_size(), m):
+        raise _bad("out overlaps x")
+    if bias is not None and _meet(at, 0, ((m - 1) * ldy + n) * size, bias.data_ptr(), 0, 4 * n, 1):
+        raise _bad("out overlaps bias")
+
+
 def _written(out):
     """out= has been written in place: a backward pass that has saved it finds that."""
     if not out.is_inference():
@@ -157,13 +176,16 @@ def _written(out):
 
 
 def int8_matmul(a: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None, dtype=torch.float32, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """y[i, j] = (sum_k a[i, k] w[j, k]) * a.scale[i] * w.scale[j] (+ bias[j]): the sum exact in int32, one rounding to dtype."""
+    """y[i, j] = (sum_k a[i, k] w[j, k]) * a.scale[i] * w.scale[j] (+ bias[j]): the sum exact in int32, one rounding to dtype.
+    out: a matrix of dtype with contiguous rows that the results are written to (apart from the inputs)."""
     device = a.device
     if device.type != "cuda":
         raise _bad("a must be on a GPU: there is no CPU path")
     m, k, n = a.rows, a.cols, w.rows
     _forward_only(a.scale, "scale")
     y, ldy = _result(w, bias, m, k, dtype, out, device)
+    if out is not None and m and n:
+        _apart(y, m, n, ldy, None, 0, 0, bias)
     nbytes = _int8_bytes(m, n, k)[0]
     ws = _workspace(nbytes, device)
     _call(hip.lib().gl3_int8_matmul, device, a.codes.data_ptr(), a.ld, a.scale.data_ptr(), w.codes.data_ptr(), w.ld, w.scale.data_ptr(), _ptr(bias), m, n, k,
@@ -172,7 +194,8 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None, d
 
 
 def int8_linear(x: torch.Tensor, w: Int8Rows, bias: Optional[torch.Tensor] = None, dtype=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """int8_matmul(quantize_rows(x), w, bias), bit for bit, in as few launches as the sizes allow.  dtype: of the result (default: x's)."""
+    """int8_matmul(quantize_rows(x), w, bias), bit for bit, in as few launches as the sizes allow.  dtype: of the result (default: x's).
+    out: as in int8_matmul."""
     ldx = _rows(x, "x")
     m, k = x.shape
     n = w.rows
@@ -180,6 +203,8 @@ def int8_linear(x: torch.Tensor, w: Int8Rows, bias: Optional[torch.Tensor] = Non
     if dtype is None:
         dtype = x.dtype
     y, ldy = _result(w, bias, m, k, dtype, out, device)
+    if out is not None and m and n:
+        _apart(y, m, n, ldy, x, ldx, k, bias)
     nbytes = _int8_bytes(m, n, k)[1]
     ws = _workspace(nbytes, device)
     _call(hip.lib().gl3_int8_linear, device, x.data_ptr(), _TYPES[x.dtype], ldx, w.codes.data_ptr(), w.ld, w.scale.data_ptr(), _ptr(bias), m, n, k,

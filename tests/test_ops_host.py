@@ -314,3 +314,17 @@ def test_scales_and_their_derivatives(hip, ops):
         with torch.no_grad(), pytest.raises(hip.Gl3Error):
             ops.Int8Rows(codes, forward_ad.make_dual(scale, torch.ones(3)), 5)
         assert ops.Int8Rows(codes, scale, 5).rows == 3
+
+
+def test_matrices_that_meet(ops):
+    """Against the bytes themselves, for small matrices; of one pitch exactly, of two pitches never too few."""
+    import itertools
+    for rows, p, pitch, width, q, pitch2, width2 in itertools.product((1, 2, 3), (0, 5), (6, 9), (1, 4, 6), range(0, 24, 1), (6, 9), (2, 5)):
+        if rows > 1 and (width > pitch or width2 > pitch2):
+            continue
+        a = {p + r * pitch + c for r in range(rows) for c in range(width)}
+        b = {q + r * pitch2 + c for r in range(rows) for c in range(width2)}
+        got = ops._meet(p, pitch, width, q, pitch2, width2, rows)
+        assert got or not a & b
+        if rows == 1 or pitch == pitch2:
+            assert got == bool(a & b), (rows, p, pitch, width, q, pitch2, width2)

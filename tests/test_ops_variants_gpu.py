@@ -298,3 +298,23 @@ def test_a_saved_tensor_that_is_written_is_noticed(ops):
     with torch.inference_mode():
         out = torch.zeros(4, 10, device=DEV)
         assert torch.equal(ops.int8_linear(x, w, out=out), ops.int8_linear(x, w))
+
+
+def test_a_result_over_an_input_is_refused(ops, hip):
+    """Results over x or the bias; columns of one buffer side by side are apart."""
+    for m in (1, 3, 40, 300):
+        buffer = torch.randn(m, 400, device=DEV)
+        x = buffer[:, :128]
+        w = int8_rows(ops, 128, 128, 1)
+        want = ops.int8_linear(x.clone(), w)
+        for out in (x, buffer[:, 100:228], buffer[:, :128]):
+            with pytest.raises(hip.Gl3Error):
+                ops.int8_linear(x, w, out=out)
+        bias = buffer.view(-1)[200:328]
+        with pytest.raises(hip.Gl3Error):
+            ops.int8_linear(x.clone(), w, bias, out=buffer[:, 180:308])
+        with pytest.raises(hip.Gl3Error):
+            ops.int8_matmul(ops.quantize_rows(x), w, bias, out=buffer[:, 180:308])
+        assert torch.equal(ops.int8_linear(x, w, out=buffer[:, 128:256]), want) and torch.equal(buffer[:, 128:256], want)
+        assert torch.equal(ops.int8_linear(x, w, out=buffer[:, 272:400]), want)
+    assert ops.int8_linear(buffer[:0, :128], w, out=buffer[:0, :128]).shape == (0, 128)
