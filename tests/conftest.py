@@ -24,7 +24,7 @@ def pytest_collection_modifyitems(config, items):
     gather's bounded spin gives up (seen once in round 3 as test 105 of 172; the same tests pass alone).  One process per GPU —
     the production layout — has one stream per process and no such coupling."""
     def tp_first(item):
-        return 0 if ("test_gpu_tp.py" in item.nodeid or "tp8" in item.nodeid) else 1
+        return 0 if ("test_gpu_tp.py" in item.nodeid or "tp8" in item.nodeid or "two_ranks" in item.nodeid) else 1
     items.sort(key=tp_first)          # stable: everything else keeps its order
 
 
