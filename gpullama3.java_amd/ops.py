@@ -184,7 +184,7 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None, d
     m, k, n = a.rows, a.cols, w.rows
     _forward_only(a.scale, "scale")
     y, ldy = _result(w, bias, m, k, dtype, out, device)
-    if out is not None and m and n:
+    if out is not None and bias is not None and m and n:
         _apart(y, m, n, ldy, None, 0, 0, bias)
     nbytes = _int8_bytes(m, n, k)[0]
     ws = _workspace(nbytes, device)
