@@ -50,7 +50,7 @@ hipError_t op_quantize(hipStream_t s, const void* x, int32_t type, int64_t rows,
 }
 
 // Which tile, and into how many parts its sum over k goes: the ones with the least estimated time.  A stage of a BM x BN tile takes a CU 0.00164 (BM + BN) us for
-// its operands' bytes + 0.0000101 BM BN us for its MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.56, 64 x 128 0.38, 32 x 128 0.30, 64 x 64 0.25), a tile 3 us and its results'
+// its operands' bytes + 0.0000101 BM BN us for its MFMAs (256 x 256 1.5, 128 x 256 0.96, 128 x 128 0.59, 64 x 128 0.40, 32 x 128 0.30, 64 x 64 0.25), a tile 3 us and its results'
 // bytes at 37 GB/s besides.  256 CUs take the workgroups in rounds; two workgroups of a small tile share a CU; the weights leave memory at 5.4 TB/s.  Tiles that are
 // too few for the CUs get their sums in parts of at least OP_PART_STAGES stages; a launch of its own adds them up, 2.5 us (on the host another 3: 4.5 here)
 // and what it reads (us, in parts / whole,

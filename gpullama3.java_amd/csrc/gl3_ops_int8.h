@@ -143,8 +143,8 @@ template <typename TY> struct OpProductArgs {
 
 // A few tokens: the weights' bytes are what it costs, and they go from memory to the matrix cores' registers directly.  A wavefront has 16 channels
 // x 16 MT tokens (v_mfma_i32_16x16x64_i8: lane l holds 16 consecutive k of row l % 16) and a ring of D steps of 64 k on their way; the KS wavefronts of a
-// workgroup share the channels and split k (their int32 sums meet in LDS: exact in any order).  The tokens' codes come from the caches, which costs
-// 4 % of the weights' time a token (128256 x 4096, us: 1 token 83 = 6.3 TB/s, 4 95, 16 144, 32 197; tiles 88, 92, 96, 96): op_streams compares.
+// workgroup share the channels and split k (their int32 sums meet in LDS: exact in any order).  The tokens' codes come from the caches again in every
+// strip, which costs 4 % of the weights' time a token (128256 x 4096, us, the least of many: 1 token 83 = 6.3 TB/s, 4 95, 16 144, 32 197; tiles 88, 92, 96, 96): op_streams compares.
 // A short k starts no loads that it does not need (100000 x 256, a step a wavefront: 31 -> 13).  (Loads past the caches fetch the 128-byte lines twice, half by half: 85 -> 95.  32 or 64 channels a wavefront: 92, 97.)
 template <int KS> struct OpStrip {          // the wavefront's part of a strip of 16 channels
     int lane, wave, r16, kg, n0, s0, cnt;
@@ -274,9 +274,11 @@ static __global__ __launch_bounds__(64 * KS) void op_token_kernel(OpProductArgs<
 // quarter, so the matrix cores have that quarter while the next stage's first fragments are read, and it waits for all loads but those that have a
 // stage left to travel.  16-byte chunk c of row r stands at chunk c ^ (r / 2 % 8): the 16 lanes of a read cover the banks once.  Workgroups go to the
 // 8 XCDs in turn; the token tiles of one channel tile run on one XCD, so its weights leave HBM once.
-// What bounds it: 32 x 128 and 64 x 128 tiles the weights (32 tokens, 151936 x 2560: 77 us, 5.05 TB/s); 256 x 256 tiles the matrix cores: a stage takes about
-// the 2048 cycles that its MFMAs issue in, at the 1.3 - 1.5 GHz that the card's power leaves (512 x 128256 x 4096 250 - 310 us from card to card, 2.1 POP/s with
-// the 1.5 - 4 us in front of a tile's first stage and the 3.3 (bfloat16) - 4.8 us (float32) of its results; a short loop of nothing but these MFMAs 4.0; 8192 x 8192 x 8192 551 us, 2.0).
+// What bounds it: 32 x 128 and 64 x 128 tiles the weights' way through LDS (32 tokens, 151936 x 2560: 76 us, 5.1 TB/s).  256 x 256 tiles: 512 x 128256 x 4096 takes
+// 255 - 310 us from card to card, 2.0 POP/s, as fast as the library's product (a short loop of nothing but these MFMAs 4.0; 8192 x 8192 x 8192 554 us, the library's 533).
+// The matrix cores are busy for 62 % of the launch's cycles (256.5 k of 413 k at 1.4 GHz; 2041 x 14336 x 4096 61 %).  Stamps in one workgroup gave 2030 MFMA cycles
+// of 2048 - 2080 a stage, 1.5 - 4 us in front of a tile's first stage and 3.3 (bfloat16) - 4.8 us (float32) for its results: four rounds of tiles make that a
+// fifth to a third of the idle cycles, and what takes the others is not known.
 // Tried: 64 k a stage with a longer ring of weights, loads by some wavefronts and MFMAs by others (62 -> 85 us at 512 x 28672 x 4096); four wavefronts of
 // 128 x 128 (same); one workgroup a CU that goes through its tiles without a pause (same); priorities, one or three reads behind an MFMA (same).
 __device__ __forceinline__ void op_dma16(const void* src, void* lds) {

@@ -194,7 +194,8 @@ def int8_matmul(a: Int8Rows, w: Int8Rows, bias: Optional[torch.Tensor] = None, d
 
 
 def int8_linear(x: torch.Tensor, w: Int8Rows, bias: Optional[torch.Tensor] = None, dtype=None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
-    """int8_matmul(quantize_rows(x), w, bias), bit for bit, in as few launches as the sizes allow.  dtype: of the result (default: x's).
+    """int8_matmul(quantize_rows(x), w, bias), bit for bit, in as few launches as the sizes allow (one up to 4 tokens, 8 where k <= 2048, of matrices that are
+    not too wide: several products of such rows want a linear each, of more rows one quantize_rows).  dtype: of the result (default: x's).
     out: as in int8_matmul."""
     ldx = _rows(x, "x")
     m, k = x.shape
