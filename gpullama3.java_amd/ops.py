@@ -149,22 +149,24 @@ def _result(w, bias, m, k, dtype, out, device):
     return out, out.stride(0)
 
 
-def _meet(p, p_pitch, p_width, q, q_pitch, q_width, rows):
-    """Whether two matrices of `rows` rows, given by address, bytes between rows and bytes of a row, share a byte (of different pitches: may share one)."""
-    if p + (rows - 1) * p_pitch + p_width <= q or q + (rows - 1) * q_pitch + q_width <= p:
+def _meet(p, p_rows, p_pitch, p_width, q, q_rows, q_pitch, q_width):
+    """Whether two matrices, each given by address, rows, bytes between rows and bytes of a row, share a byte (of different pitches: may share one)."""
+    if p + (p_rows - 1) * p_pitch + p_width <= q or q + (q_rows - 1) * q_pitch + q_width <= p:
         return False
-    if rows == 1 or p_pitch != q_pitch:
+    pitch = q_pitch if p_rows == 1 else p_pitch
+    if p_rows == q_rows == 1 or (q_rows > 1 and q_pitch != pitch):
         return True
-    gap = (q - p) % p_pitch          # columns of one buffer, side by side
-    return not (p_width <= gap and gap + q_width <= p_pitch)
+    gap = (q - p) % pitch          # columns of one buffer, side by side
+    return not (p_width <= gap and gap + q_width <= pitch)
 
 
 def _apart(out, m, n, ldy, x, ldx, k, bias):
     """Workgroups write results while others still read: out must not lie over an input."""
-    size, at = out.element_size(), out.data_ptr()
-    if x is not None and _meet(at, ldy * size, n * size, x.data_ptr(), ldx * x.element_size(), k * x.element_size(), m):
+    size = out.element_size()
+    y = (out.data_ptr(), m, ldy * size, n * size)
+    if x is not None and _meet(*y, x.data_ptr(), m, ldx * x.element_size(), k * x.element_size()):
         raise _bad("out overlaps x")
-    if bias is not None and _meet(at, 0, ((m - 1) * ldy + n) * size, bias.data_ptr(), 0, 4 * n, 1):
+    if bias is not None and _meet(*y, bias.data_ptr(), 1, 0, 4 * n):
         raise _bad("out overlaps bias")
 
 

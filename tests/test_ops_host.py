@@ -317,14 +317,18 @@ def test_scales_and_their_derivatives(hip, ops):
 
 
 def test_matrices_that_meet(ops):
-    """Against the bytes themselves, for small matrices; of one pitch exactly, of two pitches never too few."""
+    """Against the bytes themselves, for small matrices; of one pitch, or a row and a matrix beside its columns, never too few, and too many only where a row
+    would go on in one that the matrix does not have."""
     import itertools
-    for rows, p, pitch, width, q, pitch2, width2 in itertools.product((1, 2, 3), (0, 5), (6, 9), (1, 4, 6), range(0, 24, 1), (6, 9), (2, 5)):
-        if rows > 1 and (width > pitch or width2 > pitch2):
+    for rows, rows2, p, pitch, width, q, pitch2, width2 in itertools.product((1, 2, 3), (1, 2, 3), (0, 5), (6, 9), (1, 4, 6), range(0, 24), (6, 9), (2, 5)):
+        if (rows > 1 and width > pitch) or (rows2 > 1 and width2 > pitch2):
             continue
         a = {p + r * pitch + c for r in range(rows) for c in range(width)}
-        b = {q + r * pitch2 + c for r in range(rows) for c in range(width2)}
-        got = ops._meet(p, pitch, width, q, pitch2, width2, rows)
-        assert got or not a & b
-        if rows == 1 or pitch == pitch2:
+        b = {q + r * pitch2 + c for r in range(rows2) for c in range(width2)}
+        got = ops._meet(p, rows, pitch, width, q, rows2, pitch2, width2)
+        assert got or not a & b, (rows, rows2, p, pitch, width, q, pitch2, width2)
+        if rows == rows2 and (rows == 1 or pitch == pitch2):
             assert got == bool(a & b), (rows, p, pitch, width, q, pitch2, width2)
+        one, many = ((q, width2), (p, pitch, width, rows)) if rows2 == 1 else ((p, width), (q, pitch2, width2, rows2))
+        if min(rows, rows2) == 1 and many[0] <= one[0] and (one[0] - many[0]) % many[1] + one[1] <= many[1]:          # the row stands within one pitch of the matrix
+            assert got == bool(a & b), (rows, rows2, p, pitch, width, q, pitch2, width2)

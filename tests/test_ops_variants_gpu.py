@@ -317,4 +317,7 @@ def test_a_result_over_an_input_is_refused(ops, hip):
             ops.int8_matmul(ops.quantize_rows(x), w, bias, out=buffer[:, 180:308])
         assert torch.equal(ops.int8_linear(x, w, out=buffer[:, 128:256]), want) and torch.equal(buffer[:, 128:256], want)
         assert torch.equal(ops.int8_linear(x, w, out=buffer[:, 272:400]), want)
+        bias = buffer[m // 2, 128:256]          # beside the columns that are written
+        want = ops.int8_linear(x, w, bias.clone())
+        assert torch.equal(ops.int8_linear(x, w, bias, out=buffer[:, 256:384]), want)
     assert ops.int8_linear(buffer[:0, :128], w, out=buffer[:0, :128]).shape == (0, 128)
