@@ -321,3 +321,29 @@ def test_a_result_over_an_input_is_refused(ops, hip):
         want = ops.int8_linear(x, w, bias.clone())
         assert torch.equal(ops.int8_linear(x, w, bias, out=buffer[:, 256:384]), want)
     assert ops.int8_linear(buffer[:0, :128], w, out=buffer[:0, :128]).shape == (0, 128)
+
+
+def test_a_pending_error_is_not_an_operators(ops, hip):
+    """A failed HIP call of the thread that the program has dealt with: the operators behind it succeed and are right."""
+    L = hip.lib()
+    m, n, k, vocab = 20, 70, 300, 70000
+    x, w, logits = torch.randn(m, k, device=DEV), int8_rows(ops, n, k, 1), torch.randn(3, vocab, device=DEV)
+    want, scores = ops.int8_linear(x, w), ops.token_logprobs(logits, None, 4)
+    y, ent, ids, values = torch.zeros(m, n, device=DEV), torch.zeros(3, device=DEV), torch.zeros(3, 4, dtype=torch.int32, device=DEV), torch.zeros(3, 4, device=DEV)
+    codes, scale, ws = torch.zeros(m, 384, dtype=torch.int8, device=DEV), torch.zeros(m, device=DEV), torch.zeros(1 << 20, dtype=torch.uint8, device=DEV)
+    s = torch.cuda.current_stream().cuda_stream
+    torch.cuda.synchronize()
+    p = lambda t: t.data_ptr()
+    calls = [lambda: L.gl3_quantize_rows(0, s, p(x), 0, m, k, k, p(codes), 384, p(scale)),
+             lambda: L.gl3_int8_linear(0, s, p(x), 0, k, p(w.codes), w.ld, p(w.scale), None, m, n, k, p(y), 0, n, p(ws), ws.numel()),
+             lambda: L.gl3_token_logprobs(0, s, p(logits), 0, 3, vocab, vocab, None, 4, None, None, p(ent), p(ids), p(values), p(ws), ws.numel())]
+    try:
+        for call in calls:
+            assert L.hipSetDevice(1000) != 0          # pending until somebody asks
+            assert call() == 0, L.gl3_last_error(None)
+    finally:
+        L.hipGetLastError()
+    torch.cuda.synchronize()
+    a = ops.quantize_rows(x)
+    assert torch.equal(codes, a.codes) and torch.equal(scale, a.scale) and torch.equal(y, want)
+    assert torch.equal(ent, scores.entropy) and torch.equal(ids, scores.top_ids) and torch.equal(values, scores.top_logprobs)
